@@ -16,7 +16,7 @@ LIB_PATH = Path(os.environ.get("CLT_LIB", HERE / "libcltmi355.so"))  # (CLT_LIB:
 CLT_F32, CLT_BF16 = 0, 1
 CLT_DECODE_ACCUMULATE, CLT_DECODE_ROUND_ACTS = 1, 2
 
-_vp, _i64, _i32, _f32, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
+_vp, _i64, _i32, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_size_t
 
 
 class AdamTensor(C.Structure):
@@ -35,6 +35,13 @@ class DecodeSource(C.Structure):
 
 
 CLT_DECODE_MAX_SOURCES = 16
+
+
+class AdamWTensor(C.Structure):
+    """clt_adamw_tensor (include/clt_mi355.h)."""
+
+    _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp), ("v_scale", _vp), ("numel", _i64),
+                ("lr", _f64), ("weight_decay", _f64), ("p_dtype", C.c_int32), ("g_dtype", C.c_int32)]
 
 
 class RowsJob(C.Structure):
@@ -99,6 +106,10 @@ SIGNATURES = {
     "clt_fvu_grad": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i32, _vp, _f32, _vp, _vp, _i32, _vp]),
     "clt_adam_step": (_i32, [_vp, _i32, _vp, _vp, _i64, _i32, _f32, _f32, _f32, _f32, _i32, _vp]),
     "clt_signsgd_step": (_i32, [_vp, _i32, _vp, _vp, _i64, _i32, _f32, _vp]),
+    "clt_adamw_step": (_i32, [_vp, _i32, _f64, _f64, _f64, _i64, C.c_uint32, _vp]),
+    "clt_mxfp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "clt_mxfp4_dequantize": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "clt_mxfp4_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _i64, _vp]),
 }
 
 _lib = None

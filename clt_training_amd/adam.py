@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .hip_ops import _DT, _call, _stream
+from .hip_ops import _DT, _call, _stream, adamw_step
 
 import os
 
@@ -163,3 +163,88 @@ class SignSGD(Adam):
     def _launch(self, devt, n_tensors, ct, cs):
         _call("clt_signsgd_step", C.c_void_p(devt.data_ptr()), n_tensors, C.c_void_p(ct.data_ptr()),
               C.c_void_p(cs.data_ptr()), ct.numel(), CHUNK, 1.0, _stream(devt))
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) on ``clt_adamw_step``: every parameter of a group in one call, with moments that do not
+    take the parameter's type as ``Adam``'s do.  ``state_bits=32``: float32 moments, whatever the parameters are.
+    ``state_bits=8``: one byte per element and moment (the first moment and the square root of the second in e4m3, one
+    power of two for 128 elements, stochastic rounding: hip_ops.adamw_step) for every tensor of at least
+    ``min_8bit_size`` elements; smaller ones keep float32 moments.  The reference's 8-bit choice is torchao's AdamW8bit
+    (trainer.py:155-164).  ``seed`` names the random bits: two runs with the same seed round alike.  Not capturable."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
+                 state_bits: int = 32, min_8bit_size: int = 4096, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, got {state_bits}")
+        if float(lr) < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"invalid hyper-parameters: lr {float(lr)}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.min_8bit_size, self.seed = state_bits, min_8bit_size, seed
+        self._step = 0
+
+    def _moments(self, p):
+        """The state of ``p`` as hip_ops.adamw_step takes it: (first, second)."""
+        st = self.state[p]
+        if not st:
+            if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+                for name in ("exp_avg", "rms"):
+                    st[name + "_codes"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+                    st[name + "_scales"] = torch.zeros(-(-p.numel() // 128), dtype=torch.uint8, device=p.device)
+            else:
+                st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        if "exp_avg" in st:
+            return st["exp_avg"], st["exp_avg_sq"]
+        return (st["exp_avg_codes"], st["exp_avg_scales"]), (st["rms_codes"], st["rms_scales"])
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        assert closure is None
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured into a graph: every replay would repeat the same step count")
+        live = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
+        for _, ps in live:
+            for p in ps:
+                if p.grad.is_sparse or not p.is_contiguous():
+                    raise RuntimeError("AdamW needs dense gradients and contiguous parameters")
+        self._step += 1
+        calls = {}  # what one call has in common -> its tensors; groups usually differ in lr alone
+        for group, ps in live:
+            if ps:
+                key = (ps[0].device, group["betas"], group["eps"])
+                c = calls.setdefault(key, ([], [], [], [], [], []))
+                lr, wd = float(group["lr"]), float(group["weight_decay"])
+                for p in ps:
+                    m, v = self._moments(p)
+                    for to, x in zip(c, (p, p.grad, m, v, lr, wd)):
+                        to.append(x)
+        for (_, betas, eps), (ps, gs, ms, vs, lrs, wds) in calls.items():
+            adamw_step(ps, gs, ms, vs, step=self._step, lr=lrs, betas=betas, eps=eps, weight_decay=wds, seed=self.seed)
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["clt_step"] = self._step
+        return sd
+
+    def load_state_dict(self, state_dict):
+        """Moments keep the type they were saved in (the base class would cast them to the parameter's)."""
+        sd = dict(state_dict)
+        step = sd.pop("clt_step", self._step)
+        saved = sd.get("state", {})
+        params = [p for g in self.param_groups for p in g["params"]]
+        state = {}
+        for i, st in saved.items():
+            p, n = params[i], params[i].numel()
+            want = ({"exp_avg": (torch.float32, n), "exp_avg_sq": (torch.float32, n)} if "exp_avg" in st else
+                    {name + part: (torch.uint8, size) for name in ("exp_avg", "rms")
+                     for part, size in (("_codes", n), ("_scales", -(-n // 128)))})
+            for name, (dtype, size) in want.items():
+                if name not in st or st[name].numel() != size or (dtype == torch.uint8) != (st[name].dtype == torch.uint8):
+                    raise ValueError(f"AdamW: the saved state of parameter {i} does not fit ({name})")
+            state[p] = {name: st[name].detach().to(device=p.device, dtype=dtype, copy=True).contiguous()
+                        for name, (dtype, _) in want.items()}
+        super().load_state_dict({**sd, "state": {}})
+        self.state.clear()
+        self.state.update(state)
+        self._step = step

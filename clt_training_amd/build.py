@@ -10,7 +10,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libcltmi355.so"
-SOURCES = ["common.hip", "decode.hip", "segments.hip", "decode_rows.hip", "topk.hip", "encoder_gemm.hip", "encoder_gemm_fast.hip", "encoder_gemm_fast16.hip", "encoder_gemm_w8.hip", "fvu.hip", "adam.hip"]
+SOURCES = ["common.hip", "decode.hip", "segments.hip", "decode_rows.hip", "topk.hip", "encoder_gemm.hip", "encoder_gemm_fast.hip", "encoder_gemm_fast16.hip", "encoder_gemm_w8.hip", "fvu.hip", "adam.hip", "adamw.hip", "mxfp4.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # (no packed fp32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on gfx950 now and then; hipcc's
 # host pass does not know the feature and says so, which is harmless)

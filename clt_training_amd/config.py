@@ -52,6 +52,9 @@ class SparseCoderConfig(Serializable):
     coalesce_topk: Literal["none", "concat", "per-layer", "group"] = "none"
     topk_coalesced: bool = False
     use_fp8: bool = False
+    # (not in the reference) the encoder product on 4-bit microscaled operands, quantised per call; gradients are those of
+    # the full-precision inputs at the selected latents
+    use_mxfp4: bool = False
 
     @property
     def torch_dtype(self):
@@ -81,7 +84,9 @@ class TrainConfig(Serializable):
     filter_bos: bool = False
     remove_first_token: bool = False
     remove_transcoded_modules: bool = False
-    optimizer: Literal["adam", "adam8", "muon", "signum"] = "signum"
+    # "adamw" / "adamw8" (not in the reference): AdamW with moments in 32 / 8 bits, adam.AdamW
+    optimizer: Literal["adam", "adam8", "adamw", "adamw8", "muon", "signum"] = "signum"
+    weight_decay: float = 0.01  # of "adamw" / "adamw8"
     lr: Optional[float] = None
     lr_warmup_steps: int = 1000
     b1: float = 0.9

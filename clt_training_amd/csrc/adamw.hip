@@ -1,0 +1,305 @@
+// Multi-tensor AdamW for gfx950 with moments of their own width: fp32, or 8 bits with one power of two for 128 elements.
+//
+//   m <- m + (1 - b1) (g - m)          v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// HBM-bound: per element 2 sizeof(p) + sizeof(g) bytes of parameter and gradient plus 16 (fp32 moments) or 4 + 4/128 (8-bit
+// moments).  One launch takes up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device
+// memory, so nothing is uploaded, kept between calls or shared by two streams.  A workgroup owns one chunk of one tensor.
+//
+// 8-bit moments.  m and r = sqrt(v) are e4m3 (v itself spans twice the binades: a factor 2^17.8 between the largest and
+// the smallest gradient of a block is what r holds), scaled by 2^E for 128 consecutive elements: 16 lanes of 8 elements,
+// so that the block's maximum is four DPP steps inside a row of 16 lanes.  E is the least integer with max 2^-E <= 448.
+// Rounding is stochastic: with b2 = 0.999 r changes by 0.05 % a step and half a step of e4m3 is 3 to 6 %, so rounding to
+// nearest would freeze it.  The 16 random bits per value are a hash of (seed, tensor, step, element): the same call gives
+// the same bits.  r > 0 is never rounded to 0 (the update m / r would jump to m / eps).  A NaN or infinite value is
+// stored as NaN and does not count for its block's scale.
+#include <math.h>
+
+#include "common.h"
+
+namespace clt {
+namespace {
+
+constexpr int MAX_TENSORS = 40;   // records in one launch's arguments (40 x 88 bytes: the argument segment holds 4 KiB)
+constexpr int VEC = 8;            // elements per lane and pass
+constexpr int PASS = 256 * VEC;   // elements per workgroup and pass
+constexpr int BLOCK8 = 128;       // elements per scale
+
+struct Rec {
+  char* p;
+  const char* g;
+  char* m;
+  char* v;
+  uint8_t* ms;  // null: fp32 moments
+  uint8_t* vs;
+  int64_t numel;
+  float decay;      // 1 - lr wd
+  float step_size;  // lr / (1 - b1^t)
+  uint32_t key;     // hash of (seed, tensor, step)
+  uint32_t chunk0;  // first workgroup
+  int32_t p_dtype, g_dtype;
+};
+
+struct Args {
+  Rec rec[MAX_TENSORS];
+  int n;
+  int chunk_elems;
+  float c1, b2, c2, inv_sqrt_bc2, eps;  // 1 - b1, b2, 1 - b2
+};
+static_assert(sizeof(Args) <= 4096, "kernel arguments");
+
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {  // two rounds of xor-shift and multiply
+  x = (x ^ (x >> 16)) * 0x21F0AAADu;
+  x = (x ^ (x >> 15)) * 0x735A2D97u;
+  return x ^ (x >> 15);
+}
+
+// Eight elements from an address with no more than the element's own alignment (gfx950 takes dword loads at any byte).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Raw8 {
+  T e[8];
+};
+template <typename T>
+__device__ __forceinline__ void load8(const char* base, int64_t i, int n, float (&f)[8]) {
+  const T* p = reinterpret_cast<const T*>(base) + i;
+  if (n >= 8) {
+    const Raw8<T> r = *reinterpret_cast<const Raw8<T>*>(p);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = (float)r.e[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = q < n ? (float)p[q] : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(char* base, int64_t i, int n, const float (&f)[8]) {
+  T* p = reinterpret_cast<T*>(base) + i;
+  if (n >= 8) {
+    Raw8<T> r;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) r.e[q] = (T)f[q];
+    *reinterpret_cast<Raw8<T>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) p[q] = (T)f[q];
+  }
+}
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// eight e4m3 codes
+__device__ __forceinline__ void load_codes(const char* base, int64_t i, int n, float scale, float (&f)[8]) {
+  uint32_t w[2] = {0, 0};
+  if (n >= 8) {
+    const Raw8<uint8_t> r = *reinterpret_cast<const Raw8<uint8_t>*>(base + i);
+    __builtin_memcpy(w, &r, 8);
+  } else {
+    for (int q = 0; q < n; ++q) w[q >> 2] |= (uint32_t)(uint8_t)base[i + q] << (8 * (q & 3));
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false);
+    const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
+    f[4 * h] = a.x * scale, f[4 * h + 1] = a.y * scale, f[4 * h + 2] = b.x * scale, f[4 * h + 3] = b.y * scale;
+  }
+}
+__device__ __forceinline__ void store_codes(char* base, int64_t i, int n, const float (&y)[8]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // (the values are on the e4m3 grid already: the conversion is exact)
+    int t = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], t, true);
+  }
+  if (n >= 8) {
+    Raw8<uint8_t> r;
+    __builtin_memcpy(&r, w, 8);
+    *reinterpret_cast<Raw8<uint8_t>*>(base + i) = r;
+  } else {
+    for (int q = 0; q < n; ++q) base[i + q] = (char)(w[q >> 2] >> (8 * (q & 3)));
+  }
+}
+
+// maximum over a row of 16 lanes, in every lane of the row
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true)));  // row_ror:8
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true)));  // row_ror:4
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true)));  // row_ror:2
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true)));  // row_ror:1
+  return v;
+}
+
+// biased exponent E + 127 of the least E with top 2^-E <= 448 = 1.75 * 2^8, E >= -126; 0 for an empty block
+__device__ __forceinline__ int scale_code(float top) {
+  const uint32_t b = __float_as_uint(top);
+  int s = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return top > 0.f ? max(s, 1) : 0;
+}
+
+// y on the e4m3 grid, |y| <= 448: up with the probability of the part that is cut off, from 16 random bits.  Normal values
+// keep 3 bits of mantissa (20 are cut); below 2^-6 the grid is that of the first binade, reached by adding 2^-6.
+template <bool KEEP>
+__device__ __forceinline__ float stochastic(float y, uint32_t bits) {
+  const float a = fabsf(y);
+  const bool low = a < 0x1p-6f;
+  float t = low ? a + 0x1p-6f : a;
+  t = __uint_as_float((__float_as_uint(t) + (bits << 4)) & 0xfff00000u);
+  t = low ? t - 0x1p-6f : t;
+  if (KEEP) t = (t == 0.f && a > 0.f) ? 0x1p-9f : t;
+  t = a < __builtin_inff() ? t : __builtin_nanf("");
+  return __builtin_copysignf(t, y);
+}
+
+template <bool KEEP>
+__device__ __forceinline__ void quantise8(char* codes, uint8_t* scales, int64_t i, int n, const float (&x)[8],
+                                          const uint32_t (&bits)[8]) {
+  float top = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float a = fabsf(x[q]);
+    top = fmaxf(top, a < __builtin_inff() ? a : 0.f);
+  }
+  const int s = scale_code(row_max(top));
+  const float inv = __uint_as_float((uint32_t)(254 - max(s, 1)) << 23);  // 2^-E (an empty block: any)
+  float y[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) y[q] = stochastic<KEEP>(x[q] * inv, bits[q]);
+  if (n > 0) {
+    store_codes(codes, i, n, y);
+    if ((threadIdx.x & 15) == 0) scales[i / BLOCK8] = (uint8_t)s;
+  }
+}
+
+template <typename PT, typename GT, bool EIGHT>
+__device__ __forceinline__ void chunk(const Rec& t, const Args& a, int64_t start) {
+  const int64_t end = min(t.numel, start + a.chunk_elems);
+  for (int64_t i = start + (int64_t)threadIdx.x * VEC; i < start + a.chunk_elems; i += PASS) {
+    if (i - (int64_t)threadIdx.x * VEC >= end) break;  // (uniform: the lanes of a block of 128 stay together)
+    const int n = (int)max((int64_t)0, min((int64_t)VEC, end - i));
+    float p[8], g[8], m[8], v[8], r[8];
+    load8<PT>(t.p, i, n, p);
+    load8<GT>(t.g, i, n, g);
+    if constexpr (EIGHT) {
+      const float sm = n > 0 ? __uint_as_float((uint32_t)t.ms[i / BLOCK8] << 23) : 0.f;
+      const float sv = n > 0 ? __uint_as_float((uint32_t)t.vs[i / BLOCK8] << 23) : 0.f;
+      load_codes(t.m, i, n, sm, m);
+      load_codes(t.v, i, n, sv, r);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = r[q] * r[q];
+    } else {
+      load8<float>(t.m, i, n, m);
+      load8<float>(t.v, i, n, v);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      m[q] = fmaf(g[q] - m[q], a.c1, m[q]);
+      v[q] = fmaf(g[q] * a.c2, g[q], v[q] * a.b2);
+      r[q] = __builtin_amdgcn_sqrtf(v[q]);
+      // 1-ulp square root and reciprocal: the update they feed is a small part of p, and r is rounded to 4 bits
+      const float upd = m[q] * __builtin_amdgcn_rcpf(fmaf(r[q], a.inv_sqrt_bc2, a.eps));
+      p[q] = fmaf(-t.step_size, upd, p[q] * t.decay);
+    }
+    store8<PT>(t.p, i, n, p);
+    if constexpr (EIGHT) {
+      uint32_t lo[8], hi[8];
+      const uint32_t seg = (uint32_t)((uint64_t)i >> 32);
+      const uint32_t key = seg == 0 ? t.key : mix32(t.key + seg * 0x9E3779B9u);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t h = mix32(((uint32_t)i + q) ^ key);
+        lo[q] = h & 0xffffu;
+        hi[q] = h >> 16;
+      }
+      quantise8<false>(t.m, t.ms, i, n, m, lo);
+      quantise8<true>(t.v, t.vs, i, n, r, hi);
+    } else {
+      store8<float>(t.m, i, n, m);
+      store8<float>(t.v, i, n, v);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void adamw_kernel(const Args a) {
+  int lo = 0, hi = a.n - 1;  // the last tensor whose first workgroup is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.rec[mid].chunk0 <= blockIdx.x) lo = mid;
+    else hi = mid - 1;
+  }
+  const Rec& t = a.rec[lo];
+  const int64_t start = (int64_t)(blockIdx.x - t.chunk0) * a.chunk_elems;
+  const bool eight = t.ms != nullptr;
+  if (t.p_dtype == CLT_BF16) {
+    if (t.g_dtype == CLT_BF16) {
+      if (eight) chunk<bf16_t, bf16_t, true>(t, a, start);
+      else chunk<bf16_t, bf16_t, false>(t, a, start);
+    } else {
+      if (eight) chunk<bf16_t, float, true>(t, a, start);
+      else chunk<bf16_t, float, false>(t, a, start);
+    }
+  } else {
+    if (t.g_dtype == CLT_BF16) {
+      if (eight) chunk<float, bf16_t, true>(t, a, start);
+      else chunk<float, bf16_t, false>(t, a, start);
+    } else {
+      if (eight) chunk<float, float, true>(t, a, start);
+      else chunk<float, float, false>(t, a, start);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace clt
+
+using namespace clt;
+
+extern "C" int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, double b1, double b2, double eps,
+                              int64_t step, uint32_t seed, clt_stream_t stream) {
+  CLT_CHECK_ARG(n_tensors >= 0 && (n_tensors == 0 || h_tensors), "clt_adamw_step: null pointer");
+  CLT_CHECK_ARG(step >= 1, "clt_adamw_step: step is counted from 1");
+  CLT_CHECK_ARG(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0, "clt_adamw_step: betas in [0, 1), eps >= 0");
+  int64_t total = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    const clt_adamw_tensor& t = h_tensors[i];
+    CLT_CHECK_ARG(t.numel >= 0, "clt_adamw_step: tensor %d: negative size", i);
+    CLT_CHECK_ARG(valid_dtype(t.p_dtype) && valid_dtype(t.g_dtype), "clt_adamw_step: tensor %d: dtype", i);
+    CLT_CHECK_ARG(t.numel == 0 || (t.p && t.g && t.m && t.v), "clt_adamw_step: tensor %d: null pointer", i);
+    CLT_CHECK_ARG((t.m_scale == nullptr) == (t.v_scale == nullptr), "clt_adamw_step: tensor %d: one moment in 8 bits", i);
+    const uintptr_t pm = dtype_size(t.p_dtype) - 1, gm = dtype_size(t.g_dtype) - 1, mm = t.m_scale ? 0 : 3;
+    CLT_CHECK_ARG(!((uintptr_t)t.p & pm) && !((uintptr_t)t.g & gm) && !(((uintptr_t)t.m | (uintptr_t)t.v) & mm),
+                  "clt_adamw_step: tensor %d: misaligned pointer", i);
+    total += t.numel;
+  }
+  CLT_CHECK_ARG(total < (1ll << 42), "clt_adamw_step: too many elements");
+  const double bc1 = 1.0 - pow(b1, (double)step), bc2 = 1.0 - pow(b2, (double)step);
+  const int chunk_elems = 4 * PASS;
+  Args a;
+  a.chunk_elems = chunk_elems;
+  a.c1 = (float)(1.0 - b1), a.b2 = (float)b2, a.c2 = (float)(1.0 - b2);
+  a.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2)), a.eps = (float)eps;
+  a.n = 0;
+  uint64_t chunks = 0;
+  for (int i = 0; i <= n_tensors; ++i) {
+    const uint64_t mine = i < n_tensors ? ((uint64_t)h_tensors[i].numel + chunk_elems - 1) / chunk_elems : 0;
+    if (a.n && (i == n_tensors || a.n == MAX_TENSORS || chunks + mine >= (1ull << 31))) {
+      hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)chunks), dim3(256), 0, (hipStream_t)stream, a);
+      CLT_CHECK_LAUNCH("clt_adamw_step");
+      a.n = 0;
+      chunks = 0;
+    }
+    if (mine == 0) continue;
+    const clt_adamw_tensor& t = h_tensors[i];
+    Rec& r = a.rec[a.n++];
+    r.p = (char*)t.p, r.g = (const char*)t.g, r.m = (char*)t.m, r.v = (char*)t.v;
+    r.ms = t.m_scale, r.vs = t.v_scale;
+    r.numel = t.numel;
+    r.decay = (float)(1.0 - t.lr * t.weight_decay);
+    r.step_size = (float)(t.lr / bc1);
+    r.key = mix32(mix32(seed + 0x9E3779B9u * (uint32_t)(i + 1)) + (uint32_t)step);
+    r.chunk0 = (uint32_t)chunks;
+    r.p_dtype = t.p_dtype, r.g_dtype = t.g_dtype;
+    chunks += mine;
+  }
+  return CLT_OK;
+}

@@ -80,6 +80,13 @@ class FitLoop:
             pgs = [dict(params=ps, lr=torch.tensor(cfg.lr or 2e-4 / (m / (2**14)) ** 0.5))  # trainer.py:166-173
                    for ps, m in zip(param_lists, num_latents)]
             opt = adam_cls(pgs, betas=(cfg.b1, cfg.b2))
+        elif cfg.optimizer in ("adamw", "adamw8"):
+            from .adam import AdamW
+
+            pgs = [dict(params=ps, lr=torch.tensor(cfg.lr or 2e-4 / (m / (2**14)) ** 0.5))  # the rule of "adam"
+                   for ps, m in zip(param_lists, num_latents)]
+            opt = AdamW(pgs, betas=(cfg.b1, cfg.b2), weight_decay=cfg.weight_decay,
+                        state_bits=8 if cfg.optimizer == "adamw8" else 32)
         elif cfg.optimizer == "signum":
             if not cfg.force_lr_warmup:
                 # trainer.py:234-242 wraps SignSGD in schedulefree.ScheduleFreeWrapper(momentum=0.95); that package is

@@ -3,7 +3,7 @@ activation: dense GEMM + bias + ReLU + row top-k under no_grad, then an identity
 node whose backward touches only the k active latents."""
 from __future__ import annotations
 
-from typing import Literal, NamedTuple
+from typing import Literal, NamedTuple, Optional
 
 import torch
 from torch import Tensor
@@ -66,22 +66,31 @@ class FusedEncoder(torch.autograd.Function):
 
 
 def fused_encoder(input: Tensor, weight: Tensor, bias: Tensor, k: int,
-                  activation: Literal["groupmax", "topk"] = "topk", use_fp8: bool = False) -> EncoderOutput:
+                  activation: Literal["groupmax", "topk"] = "topk", use_fp8: bool = False, *,
+                  use_mxfp4: bool = False, weight_mxfp4: Optional[ops.MXFP4Tensor] = None) -> EncoderOutput:
     """input (N, D), weight (M, D), bias (M,) -> top-k (or, :373-413, groupmax) values / indices
-    (fused_encoder.py:293-309)."""
+    (fused_encoder.py:293-309).  ``use_mxfp4``: the product takes ``input`` and ``weight`` in MXFP4 (hip_ops.mxfp4_linear);
+    values and indices are those of that product, gradients go to the full-precision ``input`` and ``weight`` of the
+    selected latents as if the product had been exact.  ``weight_mxfp4``: ``weight`` quantised beforehand."""
     if activation not in ("topk", "groupmax", "batchtopk"):
         raise NotImplementedError(f"activation {activation!r}")
     if use_fp8:
         raise NotImplementedError("use_fp8 is out of scope (no BASELINE config uses it)")
+    if weight_mxfp4 is not None and (not use_mxfp4 or weight_mxfp4.shape != weight.shape):
+        raise ValueError("weight_mxfp4 is the quantised form of weight, for use_mxfp4=True")
     with torch.no_grad():
         cd = _compute_dtype(input, weight)
-        x = input if input.dtype == cd else input.to(cd)
-        W = weight if weight.dtype == cd else weight.to(cd)
+        if use_mxfp4:  # (no cast to the compute dtype first: 4 bits are cut out of what is there)
+            x = input if input.dtype in (torch.float32, torch.bfloat16) else input.float()
+            W, encode = weight_mxfp4 if weight_mxfp4 is not None else weight, ops.encode_topk_mxfp4
+        else:
+            x = input if input.dtype == cd else input.to(cd)
+            W, encode = weight if weight.dtype == cd else weight.to(cd), ops.encode_topk
         if activation == "batchtopk":  # fused_encoder.py:315-318, 204-240: row top-4k, then the batch-wide threshold
-            values, indices = ops.encode_topk(x, W, bias, 4 * k, out_dtype=cd)
+            values, indices = encode(x, W, bias, 4 * k, out_dtype=cd)
             values = ops.batch_threshold(values, k)
         else:
-            values, indices = ops.encode_topk(x, W, bias, k, out_dtype=cd, activation=activation)
+            values, indices = encode(x, W, bias, k, out_dtype=cd, activation=activation)
     indices._clt_seg = SegmentsHolder()
     values = FusedEncoder.apply(input, weight, bias, values, indices, activation)
     return EncoderOutput(top_acts=values, top_indices=indices)

@@ -648,3 +648,205 @@ def fvu_grad(y: Tensor, yhat: Tensor, mask: Optional[Tensor], l2tv: Tensor, gsca
     _call("clt_fvu_grad", _ptr(y), _dt(y), _ptr(yhat), _dt(yhat), _ptr(mask), N, d, _ptr(l2tv), float(gscale), _ptr(sc),
           _ptr(G), _DT[g_dtype], _stream(y))
     return sc, G
+
+
+# ----------------------------------------------------------------------------- MXFP4: 4-bit microscaled encoder
+def _same_device(first: Tensor, *others) -> None:
+    if not first.is_cuda:
+        raise RuntimeError("clt_training_amd ops need tensors on an MI355X GPU (there is no CPU fallback)")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _call_on(t: Tensor, name: str, *args):
+    """``_call`` on the device of ``t`` and its current stream (appended), whatever the current device is."""
+    if t.device.index == torch.cuda.current_device():
+        _call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _call(name, *args, _stream(t))
+
+
+class MXFP4Tensor:
+    """A matrix [rows, cols] in MXFP4: 32 consecutive values of a row share one scale 2^(s - 127), each value is one of
+    +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}.  ``codes`` uint8 [rows, Kp / 2] (two codes a byte, the even column in the low half) and
+    ``scales`` uint8 [rows, Kp / 32], with Kp = ``cols`` rounded up to a multiple of 128 (zero codes behind the last column).
+    s = 255 marks a block that stands for NaN."""
+
+    __slots__ = ("codes", "scales", "cols")
+
+    def __init__(self, codes: Tensor, scales: Tensor, cols: int):
+        kp = -(-cols // 128) * 128
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
+            raise TypeError("MXFP4Tensor: codes and scales are uint8 matrices")
+        if cols < 1 or codes.shape[1] != kp // 2 or scales.shape != (codes.shape[0], kp // 32):
+            raise ValueError(f"MXFP4Tensor: {cols} columns need codes [rows, {kp // 2}] and scales [rows, {kp // 32}], "
+                             f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
+            raise ValueError("MXFP4Tensor: codes and scales are contiguous and on one device")
+        self.codes, self.scales, self.cols = codes, scales, cols
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.cols))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.float32) -> Tensor:
+        """The values, [rows, cols] (bfloat16 holds each of them exactly)."""
+        if dtype not in _DT:
+            raise TypeError(f"unsupported dtype {dtype}: only float32 / bfloat16")
+        _same_device(self.codes)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            _call_on(out, "clt_mxfp4_dequantize", _ptr(self.codes), _ptr(self.scales), self.shape[0], self.cols, _ptr(out),
+                     _DT[dtype])
+        return out
+
+
+def mxfp4_quantize(x: Tensor) -> MXFP4Tensor:
+    """Rows of ``x`` [R, K] (float32 / bfloat16, unit stride along K) to MXFP4: the scale of a block of 32 is
+    2^(floor(log2 max |x|) - 2), values are rounded to nearest even and saturate at 6; a block with a NaN or an infinity
+    becomes NaN."""
+    if x.dim() != 2:
+        raise ValueError(f"mxfp4_quantize: a matrix is needed, got shape {tuple(x.shape)}")
+    dt = _dt(x)
+    _same_device(x)
+    R, K = x.shape
+    if K < 1:
+        raise ValueError("mxfp4_quantize: no columns")
+    if K > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < 0:
+        x = x.contiguous()
+    kp = -(-K // 128) * 128
+    codes = torch.empty(R, kp // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(R, kp // 32, dtype=torch.uint8, device=x.device)
+    if R:
+        _call_on(x, "clt_mxfp4_quantize", _ptr(x), dt, x.stride(0) if R > 1 else K, R, K, _ptr(codes), _ptr(scales))
+    return MXFP4Tensor(codes, scales, K)
+
+
+def mxfp4_linear(x, W: MXFP4Tensor, b: Optional[Tensor] = None, *, relu: bool = False, out_dtype=None,
+                 out: Optional[Tensor] = None) -> Tensor:
+    """act(x @ W^T + b) on 4-bit operands with fp32 accumulation: ``x`` [N, K] is a tensor (its rows are quantised here) or
+    an ``MXFP4Tensor``, ``W`` [M, K], ``b`` [M] or None; ``relu``: max(., 0), NaN stays NaN.  ``out_dtype`` defaults to the
+    dtype of ``x`` (float32 for an ``MXFP4Tensor``); ``out`` [N, M] may have any row stride."""
+    if not isinstance(W, MXFP4Tensor):
+        raise TypeError("mxfp4_linear: W is an MXFP4Tensor (mxfp4_quantize)")
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else (torch.float32 if isinstance(x, MXFP4Tensor) else x.dtype)
+    if out_dtype not in _DT:
+        raise TypeError(f"unsupported dtype {out_dtype}: only float32 / bfloat16")
+    if len(x.shape) != 2 or x.shape[1] != W.cols:
+        raise ValueError(f"mxfp4_linear: x {tuple(x.shape)} does not fit W {tuple(W.shape)}")
+    N, (M, K) = x.shape[0], W.shape
+    if b is not None:
+        if b.shape != (M,):
+            raise ValueError(f"mxfp4_linear: bias {tuple(b.shape)} for {M} rows of W")
+        b = _c(b)
+        bdt = _dt(b)
+    else:
+        bdt = 0
+    _same_device(W.codes, x.codes if isinstance(x, MXFP4Tensor) else x, b, out)
+    if out is None:
+        out = torch.empty(N, M, dtype=out_dtype, device=W.device)
+    elif out.shape != (N, M) or out.dtype != out_dtype or M > 1 and out.stride(1) != 1 or N > 1 and out.stride(0) < M:
+        raise ValueError(f"mxfp4_linear: out must be [{N}, {M}] {out_dtype} with rows that do not overlap")
+    if N == 0 or M == 0:
+        return out
+    if not isinstance(x, MXFP4Tensor):
+        x = mxfp4_quantize(x)
+    _call_on(out, "clt_mxfp4_linear", _ptr(x.codes), _ptr(x.scales), _ptr(W.codes), _ptr(W.scales), _ptr(b), bdt, N, M, K,
+             int(relu), _ptr(out), _DT[out_dtype], out.stride(0) if N > 1 else M)
+    return out
+
+
+def encode_topk_mxfp4(x: Tensor, W, b: Optional[Tensor], k: int, out_dtype=None, activation: str = "topk"):
+    """``encode_topk`` on 4-bit operands: relu(x W^T + b) through ``mxfp4_linear``, then the row top-k or groupmax.  ``W`` is
+    a table (quantised here, as a training step needs it) or an ``MXFP4Tensor`` (quantised once, for a frozen coder)."""
+    if activation not in ("topk", "groupmax"):
+        raise NotImplementedError(f"activation {activation!r}: 'topk' and 'groupmax' are on the MI355X hot path")
+    if not isinstance(W, MXFP4Tensor):
+        W = mxfp4_quantize(W)
+    N, M = x.shape[0], W.shape[0]
+    out_dtype = out_dtype or x.dtype
+    if N == 0:
+        return (torch.empty(0, k, dtype=out_dtype, device=x.device), torch.empty(0, k, dtype=torch.int64, device=x.device))
+    size = N * M * torch.empty((), dtype=out_dtype).element_size()
+    pre = workspace(x.device, size, "pre")[:size].view(out_dtype).view(N, M)
+    mxfp4_linear(x, W, b, relu=True, out=pre)
+    return (topk_rows if activation == "topk" else groupmax_rows)(pre, k, out_dtype=out_dtype)
+
+
+# ----------------------------------------------------------------------------- AdamW
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay=0.01, seed: int = 0) -> None:
+    """One AdamW step (decoupled weight decay) over lists of tensors, in place, with one launch for every 40 tensors.
+    params: float32 / bfloat16, contiguous, no two the same; grads: float32 / bfloat16 of the same shapes.
+    ``exp_avgs[i]`` and ``exp_avg_sqs[i]`` are float32 tensors of the parameter's shape, or both are pairs (codes, scales):
+    one byte per element (uint8 or float8_e4m3fn) and one byte per 128 elements (uint8 or float8_e8m0fnu) that hold the
+    first moment and the SQUARE ROOT of the second in e4m3 times a power of two (all zero bytes: zero moments), rounded
+    stochastically with random bits that ``seed``, the position in the list, ``step`` and the element determine.
+    ``lr`` and ``weight_decay`` are numbers or one number per tensor; ``step`` counts from 1."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
+        raise ValueError("adamw_step: one gradient and two moments for every parameter")
+    if n == 0:
+        return
+    dev = params[0].device
+    _same_device(params[0])
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step cannot be captured into a graph: the step count is a number of the call, and every "
+                           "replay would repeat the same step")
+    lrs = lr if isinstance(lr, (list, tuple)) else None
+    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else None
+    if lrs is not None and len(lrs) != n or wds is not None and len(wds) != n:
+        raise ValueError("adamw_step: lr and weight_decay are numbers or one number per tensor")
+    one_lr, one_wd = (0.0 if lrs is not None else float(lr)), (0.0 if wds is not None else float(weight_decay))
+    table = (_lib.AdamWTensor * n)()
+    keep, seen, live = [], set(), 0  # (keep: the contiguous copies outlive the launch)
+    for i, (r, p, g, m, v) in enumerate(zip(table, params, grads, exp_avgs, exp_avg_sqs)):
+        if p.dtype not in _DT or g.dtype not in _DT:
+            raise TypeError(f"adamw_step: tensor {i}: only float32 / bfloat16, got {p.dtype} and {g.dtype}")
+        if p.device != dev or g.device != dev or g.shape != p.shape or not p.is_contiguous():
+            raise ValueError(f"adamw_step: tensor {i}: a contiguous parameter and a gradient of its shape on {dev}")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        numel = p.numel()
+        if isinstance(m, (tuple, list)) != isinstance(v, (tuple, list)):
+            raise ValueError(f"adamw_step: tensor {i}: both moments in 32 bits or both in 8")
+        if isinstance(m, (tuple, list)):
+            (m, ms), (v, vs) = m, v
+            for c, s in ((m, ms), (v, vs)):
+                if c.dtype not in _CODES8 or s.dtype not in _SCALES8:
+                    raise TypeError(f"adamw_step: tensor {i}: 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
+                                    f"float8_e8m0fnu scales, got {c.dtype} and {s.dtype}")
+                if (c.numel() != numel or s.numel() != -(-numel // 128) or not c.is_contiguous() or not s.is_contiguous()
+                        or c.device != dev or s.device != dev):
+                    raise ValueError(f"adamw_step: tensor {i}: one code per element and one scale per 128, contiguous, on {dev}")
+            r.m_scale, r.v_scale = ms.data_ptr() or None, vs.data_ptr() or None
+        else:
+            for c in (m, v):
+                if c.dtype != torch.float32:
+                    raise TypeError(f"adamw_step: tensor {i}: moments are float32 or 8-bit pairs, got {c.dtype}")
+                if c.shape != p.shape or not c.is_contiguous() or c.device != dev:
+                    raise ValueError(f"adamw_step: tensor {i}: moments of the parameter's shape, contiguous, on {dev}")
+        r.p, r.g, r.m, r.v = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
+        r.numel = numel
+        if numel:
+            live += 1
+            seen.update((r.p, r.m, r.v))
+        r.lr = one_lr if lrs is None else float(lrs[i])
+        r.weight_decay = one_wd if wds is None else float(wds[i])
+        r.p_dtype, r.g_dtype = _DT[p.dtype], _DT[g.dtype]
+    if len(seen) != 3 * live:
+        raise ValueError("adamw_step: a tensor is given twice (parameters and moments are updated in place)")
+    _call_on(params[0], "clt_adamw_step", C.cast(table, C.c_void_p), n, float(betas[0]), float(betas[1]), float(eps),
+             int(step), int(seed) & 0xFFFFFFFF)
+
+
+_CODES8 = (torch.uint8, torch.float8_e4m3fn)
+_SCALES8 = (torch.uint8, torch.float8_e8m0fnu)

@@ -241,6 +241,7 @@ class SparseCoder(nn.Module):
         self.num_latents = cfg.num_latents or d_in * cfg.expansion_factor
         self.multi_target = cfg.n_targets > 0 and cfg.transcode
         self.mesh = None
+        self.encoder_mxfp4 = None  # (quantize_encoder)
         weight_dtype = cfg.torch_dtype
         if weight_dtype is None:
             weight_dtype = dtype
@@ -438,7 +439,16 @@ class SparseCoder(nn.Module):
         if not self.cfg.transcode:
             x = x - self.b_dec
         return fused_encoder(x, self.encoder.weight, self.encoder.bias, self.cfg.k, self.cfg.activation,
-                             self.cfg.use_fp8)
+                             self.cfg.use_fp8, use_mxfp4=self.cfg.use_mxfp4 or self.encoder_mxfp4 is not None,
+                             weight_mxfp4=self.encoder_mxfp4)
+
+    def quantize_encoder(self, on: bool = True) -> "SparseCoder":
+        """Serving: ``encode`` takes the encoder's weight as it is NOW in MXFP4 (a quarter of the bytes that every token
+        reads), whatever happens to ``encoder.weight`` later; call it again after a change.  ``on=False``: back to the
+        full-precision product.  Not part of the checkpoint.  In training mode with ``cfg.use_mxfp4`` no copy is needed:
+        each call quantises the weight it finds."""
+        self.encoder_mxfp4 = ops.mxfp4_quantize(self.encoder.weight.detach()) if on else None
+        return self
 
     def decode(self, top_acts: Tensor, top_indices: Tensor, index: int = 0) -> Tensor:
         """sparse_coder.py:649-661."""

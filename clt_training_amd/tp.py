@@ -37,6 +37,10 @@ class TPTrainer(FitLoop):
             first = next(iter(dataset))
             input_widths = {h: first[h][0].shape[-1] for h in cfg.hookpoints}
         self.saes = {}
+        if cfg.optimizer in ("adamw", "adamw8"):
+            raise NotImplementedError("AdamW's state is not gathered over latent shards: use trainer.Trainer")
+        if cfg.sae.use_mxfp4:
+            raise NotImplementedError("use_mxfp4 runs on trainer.Trainer, not on the latent-sharded engine")
         if coders is None:
             sources = []
             for position, hook in enumerate(cfg.hookpoints):  # trainer.py:113-146

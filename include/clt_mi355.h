@@ -392,6 +392,52 @@ int clt_signsgd_step(const clt_adam_tensor* tensors, int n_tensors, const int32_
                      const int64_t* chunk_start, int64_t n_chunks, int chunk_elems, float lr_factor,
                      clt_stream_t stream);
 
+/* ------------------------------------------------------------------ AdamW, moments in 32 or 8 bits
+ * Decoupled weight decay (torch.optim.AdamW; the reference's 8-bit choice is trainer.py:155-164) over many tensors:
+ *   m += (1 - b1) (g - m);  v = b2 v + (1 - b2) g^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).
+ * `h_tensors` is a HOST array, read before the call returns (records travel in the kernel arguments: one launch for every
+ * 40 tensors, no device table).  Each tensor: p in `p_dtype`, g in `g_dtype`, contiguous, aligned to their element.
+ *   m_scale == v_scale == NULL: m and v fp32 [numel].
+ *   else: m and v are e4m3 codes [numel] of m and sqrt(v), with one power of two 2^(s - 127) (one byte s, [ceil(numel /
+ *   128)]) for 128 consecutive elements: the least with max |.| 2^(127 - s) <= 448 (s = 0: all zero).  Rounded
+ *   stochastically with 16 bits of a hash of (seed, position in h_tensors, step, element) per value; sqrt(v) > 0 stays > 0;
+ *   NaN and infinite values become NaN.
+ * step is 1-based.  Same arguments, same bits.                                                                     */
+typedef struct clt_adamw_tensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  uint8_t* m_scale;
+  uint8_t* v_scale;
+  int64_t numel;
+  double lr;
+  double weight_decay;
+  int32_t p_dtype;
+  int32_t g_dtype;
+} clt_adamw_tensor;
+int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, double b1, double b2, double eps, int64_t step,
+                   uint32_t seed, clt_stream_t stream);
+
+/* ------------------------------------------------------------------ MXFP4: 4-bit microscaled encoder
+ * A matrix [R, K] in MXFP4 (OCP microscaling): 32 consecutive values of a row share one scale 2^(s - 127) (one byte s),
+ * each value is one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (sign bit 3, two exponent bits, one mantissa bit), two codes a byte,
+ * the even column in the low half.  Rows are padded with zero codes to Kp = a multiple of 128 columns:
+ *   codes [R, Kp / 2], scales [R, Kp / 32], both contiguous, codes 16-byte and scales 4-byte aligned.
+ * quantize: s - 127 = clamp(floor(log2 max |x|) - 2, -127, 127), values rounded to nearest even and saturated at 6;
+ *   a block that holds a NaN or an infinity has s = 255 and stands for NaN.  x [R, K] `x_dtype`, rows ldx elements apart.
+ * dequantize: out [R, K] `out_dtype`, contiguous; bf16 holds every value exactly.
+ * linear: out[n, m] = act(sum_k x[n, k] W[m, k] + bias[m]), fp32 accumulation, rounded once; act: ReLU (NaN stays NaN) or
+ *   nothing; bias [M] `bias_dtype` or NULL; out rows ldo >= M elements apart.                                     */
+int clt_mxfp4_quantize(const void* x, int x_dtype, int64_t ldx, int64_t R, int64_t K, uint8_t* codes, uint8_t* scales,
+                       clt_stream_t stream);
+int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t K, void* out, int out_dtype,
+                         clt_stream_t stream);
+int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                     const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K, int relu, void* out, int out_dtype,
+                     int64_t ldo, clt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
