@@ -1,10 +1,21 @@
 // MXFP4 on gfx950: quantisation of rows to 4-bit microscaled codes, the way back, and the encoder product on the codes
 // (format: include/clt_mi355.h).
+#include <type_traits>
+
 #include "common.h"
 
 namespace clt {
 namespace {
 
+#ifndef V_ORDER
+#define V_ORDER 16
+#endif
+#ifndef V_NT
+#define V_NT 0
+#endif
+#ifndef V_SCHED
+#define V_SCHED 1
+#endif
 constexpr int KPAD = 128;  // columns are padded to whole matrix-instruction steps: no bounds in the product's inner loop
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -164,6 +175,7 @@ constexpr int PANEL = 16;                        // token tiles that share their
 static_assert(BIAS_OFF + TM * 4 <= TILE_LDS && 2 * TILE_LDS <= 160 * 1024, "LDS");
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // LDS[lds_dst + 16 * lane] = *(sbase + voff)
 __device__ __forceinline__ void dma16(const uint8_t* sbase, uint32_t voff, uint32_t lds_dst) {
@@ -179,11 +191,124 @@ __device__ __forceinline__ void dma16(const uint8_t* sbase, uint32_t voff, uint3
       : "memory");
 }
 
+// The same from a buffer of `size` bytes: what lies behind its end reads as zero.
+__device__ __forceinline__ i32x4 buffer_of(const uint8_t* base, int64_t size) {
+  const uint64_t a = (uint64_t)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane((int)(uint32_t)min(size, (int64_t)0x80000000));
+  r[3] = 0x00020000;
+  return r;
+}
+__device__ __forceinline__ void dma16_buffer(const i32x4& buf, uint32_t voff, uint32_t lds_dst) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(buf), "s"(lds_dst)
+      : "memory");
+}
+
+// The same, and with four bytes a lane, for all lanes (mask -1) or none (0); all lanes are active where these stand.
+__device__ __forceinline__ void dma16_masked(const i32x4& buf, uint32_t voff, uint32_t lds_dst, int mask) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_mov_b32 exec_lo, %4\n\t"
+      "s_mov_b32 exec_hi, %4\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+      "s_mov_b64 exec, -1\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(buf), "s"(lds_dst), "s"(mask)
+      : "memory");
+}
+__device__ __forceinline__ void dma4_masked(const i32x4& buf, uint32_t voff, uint32_t lds_dst, int mask) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_mov_b32 exec_lo, %4\n\t"
+      "s_mov_b32 exec_hi, %4\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds\n\t"
+      "s_mov_b64 exec, -1\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(buf), "s"(lds_dst), "s"(mask)
+      : "memory");
+}
+
 template <int T>  // half of a stage: 64 columns
 __device__ __forceinline__ f32x16 mfma4s(const i32x4& a, const i32x4& b, const f32x16& c, int sa, int sb) {
   const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
   const i32x8 B = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 2 * T, sa, 2 * T, sb);
+}
+
+// 16 bytes to an address with the element's own alignment, past L2's lines: for stores that write whole 128-byte lines
+// (5.2 TB/s either way, and the operands stay in L2; rows of 64 bytes would reach 2.9 TB/s).
+typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void store_row16(bf16_t* to, u32x4 w) {
+  __builtin_nontemporal_store((u32x4_any2)w, reinterpret_cast<u32x4_any2*>(to));
+}
+__device__ __forceinline__ void store_row16(float* to, u32x4 w) {
+  __builtin_nontemporal_store((u32x4_any4)w, reinterpret_cast<u32x4_any4*>(to));
+}
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // one v_cvt_pk_bf16_f32
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
+// One step of a transposition of 16-byte chunks between the lanes l and l ^ 1 (or l ^ 2): lanes with that bit clear keep p and
+// take the other's p as q, the others keep q and take the other's q as p.  (DPP reads a register two slots after its write.)
+template <int XOR>
+__device__ __forceinline__ void exchange(u32x4& p, u32x4& q) {
+  u32x4 a, b;
+  const uint64_t low = XOR == 1 ? 0x5555555555555555ull : 0x3333333333333333ull;
+#define CLT_STEP(PERM)                                                                                  \
+  asm("s_mov_b64 vcc, %8\n\ts_nop 1\n\t"                                                              \
+      "v_cndmask_b32_dpp %0, %6, %4, vcc " PERM "\n\tv_cndmask_b32_dpp %1, %7, %5, vcc " PERM           \
+      "\n\ts_not_b64 vcc, vcc\n\t"                                                                     \
+      "v_cndmask_b32_dpp %2, %4, %6, vcc " PERM "\n\tv_cndmask_b32_dpp %3, %5, %7, vcc " PERM           \
+      : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3])                                              \
+      : "v"(p[d]), "v"(p[d + 1]), "v"(q[d]), "v"(q[d + 1]), "s"(low)                                    \
+      : "vcc", "scc")
+#pragma unroll
+  for (int d = 0; d < 4; d += 2) {
+    uint32_t o[4];
+    if constexpr (XOR == 1) CLT_STEP("quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf");
+    else CLT_STEP("quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf");
+    a[d] = o[0], a[d + 1] = o[1], b[d] = o[2], b[d + 1] = o[3];
+  }
+#undef CLT_STEP
+  p = a;
+  q = b;
+}
+// Eight chunks of a lane (a line of 128 bytes of its token) -> line[s]: the chunk l % 4 + 4 (l / 16 % 2) of token 4 (l / 4 % 4) + s
+// + 16 (s >> 2) of this half of the wave.
+__device__ __forceinline__ void lines_of(u32x4 (&c)[8]) {
+#pragma unroll
+  for (int g = 0; g < 8; g += 4) {
+    exchange<1>(c[g], c[g + 1]);
+    exchange<1>(c[g + 2], c[g + 3]);
+    exchange<2>(c[g], c[g + 2]);
+    exchange<2>(c[g + 1], c[g + 3]);
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const auto r = __builtin_amdgcn_permlane16_swap(c[s][d], c[s + 4][d], false, false);
+      c[s][d] = r[0], c[s + 4][d] = r[1];
+    }
 }
 
 template <typename T>
@@ -196,9 +321,15 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
   const int64_t nlt = (p.M + TM - 1) / TM, ntt = (p.N + TN - 1) / TN, ntiles = nlt * ntt;
   const int64_t xg = blockIdx.x & 7, q = ntiles >> 3, rest = ntiles & 7;
   const int64_t pos = xg * q + min(xg, rest) + (blockIdx.x >> 3);
+#if V_ORDER == 0
   const int64_t panel = pos / (nlt * PANEL), in = pos - panel * nlt * PANEL;
   const int64_t width = min((int64_t)PANEL, ntt - panel * PANEL);
   const int64_t m0 = in / width * TM, n0 = (panel * PANEL + in % width) * TN;
+#else
+  const int64_t panel = pos / (ntt * V_ORDER), in = pos - panel * ntt * V_ORDER;
+  const int64_t width = min((int64_t)V_ORDER, nlt - panel * V_ORDER);
+  const int64_t n0 = in / width * TN, m0 = (panel * V_ORDER + in % width) * TM;
+#endif
 
   // ---- loader: this wave's pieces of a stage (four of W, two of x), rows past the end read the last one again
   const int rowb = p.kp / 2, sb = p.kp / 32, nst = p.kp / KS;
@@ -243,21 +374,17 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
       dma16(low, (uint32_t)(base + off - low), lds0 + SCALE_OFF + piece * 1024);
     }
   };
-  auto read_scales = [&](int row, int c, int left, int64_t end, int lds_row) {
-    i32x4 v = *reinterpret_cast<const i32x4*>(lds + SCALE_OFF + lds_row * 16);
+  const bool last = m0 + TM >= p.M || n0 + TN >= p.N;  // this tile holds a last row: some scales may lie `back` registers off
+  auto read_scales = [&](int lds_row) { return *reinterpret_cast<const i32x4*>(lds + SCALE_OFF + lds_row * 16); };
+  auto settle = [&](i32x4 v, int row, int c, int left, int64_t end) {
     const int64_t over = (int64_t)min(row, left) * sb + 16 * c - end;
-    const int back = over > 0 ? (int)over >> 2 : 0;  // registers
-    if (__builtin_amdgcn_ballot_w64(back != 0)) {
-      i32x4 u;
-      u[0] = back == 0 ? v[0] : back == 1 ? v[1] : back == 2 ? v[2] : v[3];
-      u[1] = back == 0 ? v[1] : back == 1 ? v[2] : v[3];
-      u[2] = back == 0 ? v[2] : v[3];
-      u[3] = v[3];
-      v = u;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (int)((uint32_t)v[j] >> (8 * h));  // bytes 0 and 2: this lane's blocks of the two halves
-    return v;
+    const int back = over > 0 ? (int)over >> 2 : 0;
+    i32x4 u;
+    u[0] = back == 0 ? v[0] : back == 1 ? v[1] : back == 2 ? v[2] : v[3];
+    u[1] = back == 0 ? v[1] : back == 1 ? v[2] : v[3];
+    u[2] = back == 0 ? v[2] : v[3];
+    u[3] = v[3];
+    return u;
   };
 
   f32x16 acc[4][2] = {};
@@ -288,9 +415,22 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
       }
       if (j == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sw[i] = read_scales(wm * 128 + i * 32 + r32, s0 >> 2, wleft, wend, wm * 128 + i * 32 + r32);
+        for (int i = 0; i < 4; ++i) sw[i] = read_scales(wm * 128 + i * 32 + r32);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) sx[i] = read_scales(wn * 64 + i * 32 + r32, s0 >> 2, xleft, xend, TM + wn * 64 + i * 32 + r32);
+        for (int i = 0; i < 2; ++i) sx[i] = read_scales(TM + wn * 64 + i * 32 + r32);
+        if (last) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sw[i] = settle(sw[i], wm * 128 + i * 32 + r32, s0 >> 2, wleft, wend);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sx[i] = settle(sx[i], wn * 64 + i * 32 + r32, s0 >> 2, xleft, xend);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // bytes 0 and 2: this lane's blocks of the two halves of a stage
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sw[i][e] = (int)((uint32_t)sw[i][e] >> (8 * h));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sx[i][e] = (int)((uint32_t)sx[i][e] >> (8 * h));
+        }
       }
       const char* st = lds + slot * STAGE_BYTES;
       i32x4 A[2][4], B[2][2];
@@ -309,6 +449,18 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k) acc[i][k] = mfma4s<1>(A[1][i], B[1][k], acc[i][k], sw[i][j], sx[k][j]);
+#if V_SCHED == 1  // six reads, then one read of the second half behind each of the first matrix instructions
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int e = 0; e < 6; ++e) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 10, 0);
+#elif V_SCHED == 2
+      __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);
+#endif
       slot = slot == 2 ? 0 : slot + 1;
     }
   }
@@ -365,7 +517,12 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
           uint4 w;
         };
         if (m + VEC <= p.M) {
+#if V_NT
+          typedef uint32_t nt4 __attribute__((ext_vector_type(4), aligned(4)));
+          __builtin_nontemporal_store(__builtin_bit_cast(u32x4, w), reinterpret_cast<u32x4*>(to));
+#else
           reinterpret_cast<Row*>(to)->w = w;
+#endif
         } else {
           T e[VEC];
           __builtin_memcpy(e, &w, 16);
@@ -378,6 +535,291 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
       __builtin_amdgcn_wave_barrier();
     }
   }
+}
+
+
+// The largest problems.  One persistent workgroup of eight waves per CU computes tiles of 256 latents x 256 tokens (a wave
+// 128 x 64: 4 x 2 tiles of 32 x 32, 128 accumulators, two waves per SIMD).
+//   * A stage is 256 columns: rows of 128 bytes, whole cache lines (pieces of 64-byte rows reach half the LDS-DMA rate), 64 KiB
+//     per stage in a ring of two slots.  Chunk c of a row lies at c ^ (row / 2 % 8) ^ 4 (row / 64 % 2), so a fragment read
+//     (32 rows, one chunk each) is free of conflicts.  The DMAs go through buffers: rows behind the last one read as zeros.
+//   * A stage is four steps of eight matrix instructions.  The fragments of a step are read during the step before it, also
+//     across the stages' border: the wait for the next stage and the barrier stand before a stage's LAST step, whose
+//     fragments are in registers by then; behind it the slot is free, and the DMAs of the stage after the next one go out
+//     between the matrix instructions.  A row's last stage may be half empty: what stands there is the next row's, and counts
+//     2^-254 times (a code is never NaN).
+//   * Scales come as 16 bytes of a row for two stages, in two buffers.
+//   * The rows of W are dealt to the matrix instructions' rows so that a lane ends up with 64 consecutive latents of one token
+//     (D: lane l holds column l % 32, rows 8 g + 4 (l / 32) + j).  Their 16-byte chunks are exchanged in registers, between the
+//     four lanes of a quad and between neighbouring rows of 16 lanes: a store instruction then writes whole lines of 128
+//     bytes, and the epilogue needs neither LDS nor a barrier.  The stores are issued behind the DMAs that the next tile waits
+//     for, and drain while that tile runs.
+constexpr int BM = 256, BN = 256, BK = 256;
+constexpr int BSLOT = (BM + BN) * 128, BSCALE_OFF = 2 * BSLOT, BSCALE = (BM + BN) * 16;
+constexpr int BBIAS_OFF = BSCALE_OFF + 2 * BSCALE, BIG_LDS = BBIAS_OFF + 3 * BM * 4;
+static_assert(BIG_LDS <= 160 * 1024, "LDS");
+
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef int i32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+
+struct Frags {
+  i32x4 a[4], b[2];
+};
+
+template <typename T, bool RELU>
+__global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[BIG_LDS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, h = lane >> 5, wm = wave >> 2, wn = wave & 3;
+  const int rowb = p.kp / 2, sb = p.kp / 32, nst = (p.kp + BK - 1) / BK;
+  const bool half = p.kp % BK != 0;  // the last stage has 128 columns
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+
+  // ---- tiles of this workgroup: its XCD (id % 8) owns a contiguous range of positions, a panel of latent tiles runs through
+  //      all tokens, latents fastest: the rows that an XCD writes at a time are long and its operands stay in its L2
+  const int nlt = (int)((p.M + BM - 1) / BM), ntt = (int)((p.N + BN - 1) / BN);
+  const int ntiles = nlt * ntt;  // (host: < 2^31)
+  const int xg = blockIdx.x & 7, nbx = ((int)gridDim.x - xg + 7) >> 3;
+  const int q = ntiles >> 3, rest = ntiles & 7;
+  const int xstart = xg * q + min(xg, rest), xstop = xstart + q + (xg < rest);
+  int pos = xstart + (blockIdx.x >> 3);
+  if (pos >= xstop) return;
+  auto place = [&](int at, int64_t& m0, int64_t& n0) {
+    const uint32_t full = (uint32_t)ntt * V_ORDER;
+    const uint32_t panel = (uint32_t)at / full, in = (uint32_t)at - panel * full;
+    const uint32_t width = min((uint32_t)V_ORDER, (uint32_t)nlt - panel * V_ORDER);
+    const uint32_t row = in / width;
+    n0 = (int64_t)__builtin_amdgcn_readfirstlane(row) * BN;
+    m0 = (int64_t)__builtin_amdgcn_readfirstlane(panel * V_ORDER + in - row * width) * BM;
+  };
+
+  // ---- loader: runs two stages ahead of the multiplier.  What lies behind an array's end reads as zero (dword by dword).
+  const bool bias_dma = p.bias && p.bias_dtype == CLT_F32;
+  i32x4 wbuf, xbuf, sbuf_, bbuf;  // from the tile's first row: codes, this wave's scales (waves 0 .. 3: W, 4 .. 7: x), bias
+  int lpos = pos, ls = 0, lslot = 0, lsbuf = 0, lbias = 0;  // the stage to be fetched next and where to
+  const uint32_t chunk = ((lane & 7) ^ (lane >> 4) ^ (2 * wave & 4)) << 4;  // (row / 2 % 8 = lane / 16, + 4 in an odd piece)
+  const uint32_t even = (uint32_t)(32 * wave + (lane >> 3)) * rowb + chunk, odd_ = even - chunk + (chunk ^ 64);
+  const uint32_t srow = (uint32_t)((wave & 3) * 64 + lane) * sb;
+  auto aim = [&]() {
+    if (lpos >= xstop) {  // nothing more to fetch: every later piece reads zeros
+      wbuf[2] = xbuf[2] = sbuf_[2] = bbuf[2] = 0;
+      return;
+    }
+    int64_t m0, n0;
+    place(lpos, m0, n0);
+    wbuf = buffer_of(p.wc + m0 * rowb, (p.M - m0) * rowb);
+    xbuf = buffer_of(p.xc + n0 * rowb, (p.N - n0) * rowb);
+    sbuf_ = wave < 4 ? buffer_of(p.ws + m0 * sb, (p.M - m0) * sb) : buffer_of(p.xs + n0 * sb, (p.N - n0) * sb);
+    bbuf = buffer_of(reinterpret_cast<const uint8_t*>(p.bias) + m0 * 4, bias_dma ? (p.M - m0) * 4 : 0);
+  };
+  auto load_piece = [&](int i) {  // 0 .. 3: W, 4 .. 7: x
+    dma16_buffer(i < 4 ? wbuf : xbuf, ((i & 1) ? odd_ : even) + (uint32_t)(ls * 128 + (i & 3) * 8 * rowb),
+                 lds0 + lslot * BSLOT + wave * 4096 + (i >> 2) * (BM * 128) + (i & 3) * 1024);
+  };
+  // (no branches in what stands between matrix instructions: the compiler would move those behind them)
+  auto load_scales = [&]() {  // with every other stage; and with a tile's first stage its bias (64 latents a wave, twice)
+    const int now = uni(~ls & 1), tile0 = uni(ls == 0 && bias_dma);
+    dma16_masked(sbuf_, srow + 8 * ls, lds0 + BSCALE_OFF + lsbuf * BSCALE + wave * 1024, -now);
+    dma4_masked(bbuf, ((wave & 3) * 64 + lane) * 4, lds0 + BBIAS_OFF + lbias * (BM * 4) + (wave & 3) * 256, -tile0);
+    lsbuf ^= now;
+    lbias = lbias + tile0 == 3 ? 0 : lbias + tile0;
+  };
+  auto advance = [&]() {
+    lslot ^= 1;
+    if (++ls == nst) {
+      ls = 0;
+      lpos += nbx;
+      aim();
+    }
+  };
+
+  // ---- multiplier
+  // this lane's row of W (+ 16 i in row tile i) and its byte in step 0; step t is at byte ^ 32 t
+  const int wrow = wm * 128 + (r32 >> 2 & 1) * 64 + (r32 >> 3) * 4 + (r32 & 3), xrow = wn * 64 + r32;
+  const uint32_t wat = wrow * 128 + ((h ^ (wrow >> 1 & 7) ^ (wrow >> 4 & 4)) << 4);
+  const uint32_t xat = BM * 128 + xrow * 128 + ((h ^ (xrow >> 1 & 7) ^ (xrow >> 4 & 4)) << 4);
+  f32x16 acc[4][2];
+  Frags F0, F1;
+  i32x2 raw[6], sc[6];  // scales of four row tiles of W and two of x: as read, and with this lane's blocks in bytes 0 and 2
+  auto read_frag = [&](Frags& f, int e, const char* base, int t) {  // in the order of their use
+    const char* a = base + (wat ^ (32 * t));
+    const char* b = base + (xat ^ (32 * t));
+    if (e == 0) f.b[0] = *reinterpret_cast<const i32x4*>(b);
+    if (e == 1) f.a[0] = *reinterpret_cast<const i32x4*>(a);
+    if (e == 2) f.b[1] = *reinterpret_cast<const i32x4*>(b + 4096);
+    if (e >= 3) f.a[e - 2] = *reinterpret_cast<const i32x4*>(a + (e - 2) * 2048);
+  };
+  auto read_scales = [&](int s, int buf) {
+    const char* base = lds + BSCALE_OFF + buf * BSCALE + 8 * (s & 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const i32x2*>(base + (wrow + 16 * i) * 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) raw[4 + i] = *reinterpret_cast<const i32x2*>(base + (BM + xrow + 32 * i) * 16);
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  // Step t of a stage: eight matrix instructions on `cur` (to: acc = instead of acc +=, a tile's first); between them the
+  // fragments of the next step come in and, if `piece` >= 0, four pieces go out.
+  auto step = [&](auto t_, auto first_, auto piece_, const Frags& cur, Frags& nxt, const char* base, int tn) {
+    constexpr int t = decltype(t_)::value, piece = decltype(piece_)::value;
+    constexpr bool first = decltype(first_)::value;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f32x16& c = acc[e >> 1][e & 1];
+      c = mfma4s<t & 1>(cur.a[e >> 1], cur.b[e & 1], first ? f32x16{} : c, sc[e >> 1][t >> 1], sc[4 + (e & 1)][t >> 1]);
+      if (e < 6) read_frag(nxt, e, base, tn);
+      if (piece >= 0 && (e & 1)) load_piece(piece + (e >> 1));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto pin = [&]() {  // the sums are computed here, not further down
+    asm volatile("" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[2][0]), "+v"(acc[2][1]),
+                 "+v"(acc[3][0]), "+v"(acc[3][1]));
+  };
+  using None = std::integral_constant<int, -1>;
+  using P0 = std::integral_constant<int, 0>;
+  using P4 = std::integral_constant<int, 4>;
+
+  int64_t m0, n0;
+  place(pos, m0, n0);
+  aim();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {  // (the second stage is half on its way when the loop begins: see `stage`)
+    load_scales();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load_piece(i);
+    advance();
+  }
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  int slot = 0, sbuf = 0;  // of the stage that is multiplied
+  int tile = 0;            // modulo 3: the loader is up to two tiles ahead, so that three biases are there at a time
+  read_scales(0, 0);
+#pragma unroll
+  for (int e = 0; e < 6; ++e) read_frag(F0, e, lds, 0);
+
+  T* out = reinterpret_cast<T*>(p.out);
+  constexpr int VEC = 16 / sizeof(T), NSTORE = 8 * sizeof(T);
+  const int nl = wn * 64 + 4 * (lane >> 2 & 3);  // the token and the latent (in the tile) of this lane's first store
+  const int ml = wm * 128 + 64 * h + ((lane >> 4 & 1) * 4 + (lane & 3)) * VEC;
+  const uint32_t lane_out = (uint32_t)(nl * (int)p.ldo + ml) * (uint32_t)sizeof(T);
+  float* bias = reinterpret_cast<float*>(lds + BBIAS_OFF);
+  if (!bias_dma) {
+    for (int i = threadIdx.x; i < 3 * BM; i += 512) bias[i] = 0.f;
+  }
+
+  for (;;) {
+    auto stage = [&](int s, auto first_) {
+      constexpr bool first = decltype(first_)::value;
+      const bool final = s == nst - 1;
+      const char* st = lds + slot * BSLOT;
+      const char* sn = lds + (slot ^ 1) * BSLOT;
+      const int s1 = final ? 0 : s + 1, sbuf1 = (s1 & 1) ? sbuf : sbuf ^ 1;
+      const bool cut = half && final;
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        sc[i][0] = (int)((uint32_t)raw[i][0] >> (8 * h));
+        sc[i][1] = cut ? 0 : (int)((uint32_t)raw[i][1] >> (8 * h));
+      }
+      if constexpr (first) {  // (its successor's pieces went out in front of the stores)
+        step(I0{}, std::true_type{}, None{}, F0, F1, st, 1);
+      } else {
+        step(I0{}, std::false_type{}, P4{}, F0, F1, st, 1);
+        pin();
+        advance();
+      }
+      step(I1{}, std::false_type{}, None{}, F1, F0, st, 2);
+      step(I2{}, std::false_type{}, None{}, F0, F1, st, 3);
+      pin();
+      // The next stage is there, and every wave has what it needs of this one.  (In a tile's first stage nothing has been
+      // issued behind the stores of the tile before; what stands in front of them is what is waited for.)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(first ? NSTORE : 0) : "memory");
+      read_scales(s1, sbuf1);
+      load_scales();
+      step(I3{}, std::false_type{}, P0{}, F1, F0, sn, 0);
+      pin();
+      slot ^= 1;
+      sbuf = sbuf1;
+    };
+    stage(0, std::true_type{});
+#pragma unroll 1
+    for (int s = 1; s < nst; ++s) stage(s, std::false_type{});
+#pragma unroll
+    for (int i = 4; i < 8; ++i) load_piece(i);
+    advance();
+
+    // ---- epilogue: bias, ReLU, one rounding.  acc[i][k][4 g + j]: token 32 k + l % 32, latent 64 h + 16 i + 4 g + j
+    if (p.bias && !bias_dma) {
+      __syncthreads();
+      if (threadIdx.x < BM) {
+        const int64_t m = m0 + threadIdx.x;
+        bias[tile * BM + threadIdx.x] = m < p.M ? load_scalar(p.bias, p.bias_dtype, m) : 0.f;
+      }
+      __syncthreads();
+    }
+    const float* bt = bias + tile * BM + wm * 128 + 64 * h;
+    const bool whole = m0 + BM <= p.M && n0 + BN <= p.N;
+    char* tile_out = reinterpret_cast<char*>(out + n0 * p.ldo + m0);  // (host: 256 rows are less than 2 GiB)
+    const int nleft = (int)min(p.N - n0, (int64_t)BN), mleft = (int)min(p.M - m0, (int64_t)BM);
+    auto finish = [&](auto whole_) {
+#pragma unroll
+      for (int part = 0; part < (int)sizeof(T) / 2; ++part) {  // 128 bytes of every token: 64 or 32 latents of each half
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          u32x4 c[8];
+#pragma unroll
+          for (int e = 0; e < 16 / (int)sizeof(T) * 2; ++e) {  // groups of four latents
+            const int i = part * 2 + e / 4, g = e % 4;
+            const float4 b = *reinterpret_cast<const float4*>(bt + 16 * i + 4 * g);
+            const f32x16& a = acc[i][k];
+            float v[4] = {a[4 * g] + b.x, a[4 * g + 1] + b.y, a[4 * g + 2] + b.z, a[4 * g + 3] + b.w};
+            if (RELU) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] = __builtin_elementwise_maximum(v[q], 0.f);
+            }
+            if constexpr (sizeof(T) == 2) {
+              c[e / 2][e % 2 * 2] = pack2(v[0], v[1]);
+              c[e / 2][e % 2 * 2 + 1] = pack2(v[2], v[3]);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) c[e][q] = __float_as_uint(v[q]);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          lines_of(c);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int s = 0; s < 8; ++s) {
+            const int n = 32 * k + 16 * (s >> 2) + (s & 3), m = part * 32;  // how far this line is from the lane's first one
+            T* to = reinterpret_cast<T*>(tile_out + (uint32_t)(n * (int)p.ldo + m) * (uint32_t)sizeof(T) + lane_out);
+            if (decltype(whole_)::value) {
+              store_row16(to, c[s]);
+            } else if (nl + n < nleft) {
+              if (ml + m + VEC <= mleft) {
+                store_row16(to, c[s]);
+              } else {
+                T e[VEC];
+                const u32x4 w = c[s];
+                __builtin_memcpy(e, &w, 16);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q)
+                  if (ml + m + q < mleft) to[q] = e[q];
+              }
+            }
+          }
+        }
+      }
+    };
+    if (whole) finish(std::true_type{});
+    else finish(std::false_type{});
+    pos += nbx;
+    if (pos >= xstop) break;
+    place(pos, m0, n0);
+    if (!whole) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (fewer stores than the next stage's wait counts on)
+    tile = tile == 2 ? 0 : tile + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (no DMA is under way when the LDS goes to another workgroup)
 }
 
 }  // namespace
@@ -436,6 +878,14 @@ extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales,
                     !((uintptr_t)out & (dtype_size(out_dtype) - 1)),
                 "clt_mxfp4_linear: misaligned pointer");
   LinearArgs a{x_codes, x_scales, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu};
+  const int64_t big = (M + BM - 1) / BM * ((N + BN - 1) / BN);
+  if (big >= 256 && big < (1ll << 31) && 256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
+    const auto kernel = out_dtype == CLT_BF16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
+                                              : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
+    hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, (hipStream_t)stream, a);
+    CLT_CHECK_LAUNCH("clt_mxfp4_linear");
+    return CLT_OK;
+  }
   const int64_t tiles = (M + TM - 1) / TM * ((N + TN - 1) / TN);
   if (N >= 16 && M >= 16 && tiles >= 64 && tiles < (1ll << 31)) {
     if (out_dtype == CLT_BF16)

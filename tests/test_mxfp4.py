@@ -203,6 +203,15 @@ def test_linear_shapes(N, M, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [32, 100, 200, 300, 500, 512, 600, 770, 1100])
+def test_linear_many_tiles(K):
+    """Problems of several hundred tiles, with rows and columns left over, and every way a row's columns can end."""
+    check_linear(2100, 9000, K, torch.bfloat16, torch.bfloat16, torch.float32, True, K)
+    check_linear(4096 + 17, 4096 + 40, K, torch.bfloat16, torch.float32, torch.bfloat16, False, K + 1)
+    check_linear(300, 40001, K, torch.float32, torch.bfloat16, None, True, K + 2, spread=3.0)
+
+
+@pytest.mark.gpu
 def test_linear_special_values():
     """NaN blocks reach every output of their row and no other; ReLU keeps NaN; the scales' ends meet in the product."""
     from clt_training_amd import hip_ops as ops
