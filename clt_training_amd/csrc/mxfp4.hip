@@ -130,6 +130,118 @@ struct LinearArgs {
   int kp, bias_dtype, relu;
 };
 
+// Few tokens (at most 16 NT): bound by reading W, so W goes from memory to registers once and nothing else is in the way.  A wave
+// takes 16 rows of W at a time (v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, columns 32 (l / 16) .. + 31 of 128),
+// with the loads of the next 512 columns -- of the next rows, at a row's end -- in flight while it multiplies.  The tokens
+// lie in LDS, quantised there by every workgroup for itself when they are so few that this is cheaper than a launch (XT: float /
+// bf16), else copied (XT: uint8_t).  Row pitch kp / 2 + 16 bytes: the 16 lanes of a fragment read hit different banks.
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+__device__ __forceinline__ f32x4 mfma4_16(const i32x4& a, const i32x4& b, const f32x4& c, int sa, int sb) {
+  const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+  const i32x8 B = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
+}
+// (what lies behind `size` reads as zero, dword by dword)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* base, int64_t size) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)max(min(size, (int64_t)0x7fffffff), (int64_t)0), 0x00020000);
+}
+
+template <typename XT, typename T, int NT>
+__global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, const XT* __restrict__ x, int64_t ldx, int K) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int rowb = p.kp / 2, sb = p.kp / 32, pitch = rowb + 16, nks = p.kp / 128;
+  const int N = (int)p.N;
+  char* xs = lds + NT * 16 * pitch;  // scales, sb bytes a row
+  if constexpr (sizeof(XT) == 1) {
+    for (int i = threadIdx.x; i < N * (rowb / 16); i += 256) {
+      const int row = i / (rowb / 16), c = i - row * (rowb / 16);
+      *reinterpret_cast<uint4*>(lds + row * pitch + 16 * c) = reinterpret_cast<const uint4*>(p.xc)[i];
+    }
+    for (int i = threadIdx.x; i < N * (sb / 4); i += 256) reinterpret_cast<uint32_t*>(xs)[i] = reinterpret_cast<const uint32_t*>(p.xs)[i];
+  } else {
+    const int lpr = p.kp / 8;  // (a multiple of 16: the four lanes of a block go the same way)
+    for (int i = threadIdx.x; i < N * lpr; i += 256) {
+      const int row = i / lpr, c = i - row * lpr;
+      float f[8];
+      load_row8(x + row * ldx, 8 * c, K, f);
+      int s;
+      *reinterpret_cast<uint32_t*>(lds + row * pitch + 4 * c) = quantise_lane(f, s);
+      if ((c & 3) == 0) xs[row * sb + c / 4] = (char)s;
+    }
+  }
+  __syncthreads();
+
+  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+  const int64_t groups = (p.M + 15) / 16, step = (int64_t)gridDim.x * 4;
+  const int nch = (nks + 3) / 4;  // pieces of 512 columns
+  int64_t g = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (g >= groups) return;
+  struct Piece {
+    u32x4 w[4], s;
+  };
+  auto load = [&](int64_t group, int c, Piece& v) {
+    const auto codes = resource(p.wc + group * 16 * rowb, (p.M - group * 16) * rowb);
+    const auto scales = resource(p.ws + group * 16 * sb, (p.M - group * 16) * sb);
+    v.s = __builtin_amdgcn_raw_buffer_load_b128(scales, r16 * sb + 16 * c, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (4 * c + j < nks) v.w[j] = __builtin_amdgcn_raw_buffer_load_b128(codes, r16 * rowb + 256 * c + 64 * j + 16 * q, 0, 0);
+  };
+  T* out = reinterpret_cast<T*>(p.out);
+  Piece now, then;
+  load(g, 0, now);
+  while (g < groups) {
+    const int64_t m = g * 16 + 4 * q;  // this lane's four latents
+    float b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = p.bias ? load_scalar(p.bias, p.bias_dtype, min(m + i, p.M - 1)) : 0.f;
+    f32x4 acc[NT] = {};
+    const int64_t next = g + step;
+    for (int c = 0; c < nch; ++c) {
+      if (c + 1 < nch) load(g, c + 1, then);
+      else if (next < groups) load(next, 0, then);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (4 * c + j >= nks) break;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const i32x4 xf = *reinterpret_cast<const i32x4*>(lds + (16 * t + r16) * pitch + 256 * c + 64 * j + 16 * q);
+          const uint32_t xsc = *reinterpret_cast<const uint32_t*>(xs + (16 * t + r16) * sb + 16 * c + 4 * j);
+          acc[t] = mfma4_16(__builtin_bit_cast(i32x4, now.w[j]), xf, acc[t], (int)(now.s[j] >> (8 * q)), (int)(xsc >> (8 * q)));
+        }
+      }
+      now = then;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = 16 * t + r16;
+      if (n >= N) continue;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = acc[t][i] + b[i];
+        if (p.relu) v[i] = __builtin_elementwise_maximum(v[i], 0.f);
+      }
+      T* to = out + n * p.ldo + m;
+      if (m + 4 <= p.M) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Four {
+          T e[4];
+        };
+        Four o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.e[i] = (T)v[i];
+        *reinterpret_cast<Four*>(to) = o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (m + i < p.M) to[i] = (T)v[i];
+      }
+    }
+    g = next;
+  }
+}
+
 // One wave per 32 latents x 32 tokens, operands straight from memory.
 template <typename T>
 __global__ __launch_bounds__(64) void mxfp4_linear_kernel(const LinearArgs p) {
@@ -866,18 +978,55 @@ extern "C" int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
   return CLT_OK;
 }
 
+namespace {
+
+constexpr int FEW_LDS = 64 * 1024;
+int few_lds(int nt, int kp) { return nt * 16 * (kp / 2 + 16 + kp / 32); }
+// 16, 32 or 64 tokens of kp columns in LDS (0: too many)
+int few_tiles(int64_t N, int kp) {
+  const int nt = N <= 16 ? 1 : N <= 32 ? 2 : N <= 64 ? 4 : 0;
+  return nt && few_lds(nt, kp) <= FEW_LDS ? nt : 0;
+}
+// So few values of x that every workgroup of the product quantises them for itself.
+bool few_raw(int64_t N, int64_t K) { return few_tiles(N, (int)((K + KPAD - 1) / KPAD * KPAD)) && N * K <= 8192; }
+
+template <typename XT, typename T>
+void launch_few(const LinearArgs& a, const XT* x, int64_t ldx, int64_t K, hipStream_t st) {
+  const int nt = few_tiles(a.N, a.kp), lds = few_lds(nt, a.kp);
+  const int64_t blocks = (a.M + 127) / 128;  // two groups of 16 rows and more a wave
+  const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
+  const auto kernel = nt == 1 ? mxfp4_few_kernel<XT, T, 1> : nt == 2 ? mxfp4_few_kernel<XT, T, 2> : mxfp4_few_kernel<XT, T, 4>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, x, ldx, (int)K);
+}
+
+int check_linear(const char* name, const void* w_codes, const void* w_scales, const void* bias, int bias_dtype, int64_t N,
+                 int64_t M, int64_t K, const void* out, int out_dtype, int64_t ldo) {
+  CLT_CHECK_ARG(w_codes && w_scales && out, "%s: null pointer", name);
+  CLT_CHECK_ARG(valid_dtype(out_dtype) && (!bias || valid_dtype(bias_dtype)), "%s: dtype", name);
+  CLT_CHECK_ARG(N > 0 && M > 0 && K > 0 && ldo >= M, "%s: bad sizes", name);
+  CLT_UNSUPPORTED(N <= 32 * 65535ll && M < (1ll << 31) && K < (1ll << 24), "%s: N <= %lld, M < 2^31, K < 2^24", name, 32 * 65535ll);
+  CLT_CHECK_ARG(aligned16(w_codes) && !((uintptr_t)w_scales & 3) && !((uintptr_t)out & (dtype_size(out_dtype) - 1)) &&
+                    !(bias && ((uintptr_t)bias & (dtype_size(bias_dtype) - 1))),
+                "%s: misaligned pointer", name);
+  return CLT_OK;
+}
+
+}  // namespace
+
 extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes,
                                 const uint8_t* w_scales, const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K,
                                 int relu, void* out, int out_dtype, int64_t ldo, clt_stream_t stream) {
-  CLT_CHECK_ARG(x_codes && x_scales && w_codes && w_scales && out, "clt_mxfp4_linear: null pointer");
-  CLT_CHECK_ARG(valid_dtype(out_dtype) && (!bias || valid_dtype(bias_dtype)), "clt_mxfp4_linear: dtype");
-  CLT_CHECK_ARG(N > 0 && M > 0 && K > 0 && ldo >= M, "clt_mxfp4_linear: bad sizes");
-  CLT_UNSUPPORTED(N <= 32 * 65535ll && M < (1ll << 31) && K < (1ll << 24), "clt_mxfp4_linear: N <= %lld, M < 2^31, K < 2^24",
-                  32 * 65535ll);
-  CLT_CHECK_ARG(aligned16(x_codes) && aligned16(w_codes) && !((uintptr_t)x_scales & 3) && !((uintptr_t)w_scales & 3) &&
-                    !((uintptr_t)out & (dtype_size(out_dtype) - 1)),
-                "clt_mxfp4_linear: misaligned pointer");
+  const int rc = check_linear("clt_mxfp4_linear", w_codes, w_scales, bias, bias_dtype, N, M, K, out, out_dtype, ldo);
+  if (rc) return rc;
+  CLT_CHECK_ARG(x_codes && x_scales, "clt_mxfp4_linear: null pointer");
+  CLT_CHECK_ARG(aligned16(x_codes) && !((uintptr_t)x_scales & 3), "clt_mxfp4_linear: misaligned pointer");
   LinearArgs a{x_codes, x_scales, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu};
+  if (few_tiles(N, a.kp)) {
+    if (out_dtype == CLT_BF16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, (hipStream_t)stream);
+    else launch_few<uint8_t, float>(a, nullptr, 0, K, (hipStream_t)stream);
+    CLT_CHECK_LAUNCH("clt_mxfp4_linear");
+    return CLT_OK;
+  }
   const int64_t big = (M + BM - 1) / BM * ((N + BN - 1) / BN);
   if (big >= 256 && big < (1ll << 31) && 256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
     const auto kernel = out_dtype == CLT_BF16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
@@ -902,4 +1051,40 @@ extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales,
     hipLaunchKernelGGL(mxfp4_linear_kernel<float>, grid, dim3(64), 0, (hipStream_t)stream, a);
   CLT_CHECK_LAUNCH("clt_mxfp4_linear");
   return CLT_OK;
+}
+
+extern "C" size_t clt_mxfp4_linear_x_workspace_bytes(int64_t N, int64_t K) {
+  if (N <= 0 || K <= 0 || few_raw(N, K)) return 0;
+  return align_up((size_t)N * (padded(K) / 2), 16) + (size_t)N * (padded(K) / 32);
+}
+
+extern "C" int clt_mxfp4_linear_x(const void* x, int x_dtype, int64_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
+                                  const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K, int relu, void* out,
+                                  int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes, clt_stream_t stream) {
+  const int rc = check_linear("clt_mxfp4_linear_x", w_codes, w_scales, bias, bias_dtype, N, M, K, out, out_dtype, ldo);
+  if (rc) return rc;
+  CLT_CHECK_ARG(x && valid_dtype(x_dtype) && ldx >= 0 && !((uintptr_t)x & (dtype_size(x_dtype) - 1)),
+                "clt_mxfp4_linear_x: x is null or misaligned, or its dtype or stride is wrong");
+  if (few_raw(N, K)) {
+    const LinearArgs a{nullptr, nullptr, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu};
+    const hipStream_t st = (hipStream_t)stream;
+    if (x_dtype == CLT_BF16) {
+      if (out_dtype == CLT_BF16) launch_few<bf16_t, bf16_t>(a, (const bf16_t*)x, ldx, K, st);
+      else launch_few<bf16_t, float>(a, (const bf16_t*)x, ldx, K, st);
+    } else {
+      if (out_dtype == CLT_BF16) launch_few<float, bf16_t>(a, (const float*)x, ldx, K, st);
+      else launch_few<float, float>(a, (const float*)x, ldx, K, st);
+    }
+    CLT_CHECK_LAUNCH("clt_mxfp4_linear_x");
+    return CLT_OK;
+  }
+  const size_t need = clt_mxfp4_linear_x_workspace_bytes(N, K);
+  if (!workspace || workspace_bytes < need) {
+    set_error("clt_mxfp4_linear_x: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
+    return CLT_ERR_WORKSPACE;
+  }
+  uint8_t* codes = (uint8_t*)workspace;
+  uint8_t* scales = codes + align_up((size_t)N * (padded(K) / 2), 16);
+  const int q = clt_mxfp4_quantize(x, x_dtype, ldx, N, K, codes, scales, stream);
+  return q ? q : clt_mxfp4_linear(codes, scales, w_codes, w_scales, bias, bias_dtype, N, M, K, relu, out, out_dtype, ldo, stream);
 }

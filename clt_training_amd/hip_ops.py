@@ -6,6 +6,7 @@ if the tensors are not on a GPU."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -652,20 +653,23 @@ def fvu_grad(y: Tensor, yhat: Tensor, mask: Optional[Tensor], l2tv: Tensor, gsca
 
 # ----------------------------------------------------------------------------- MXFP4: 4-bit microscaled encoder
 def _same_device(first: Tensor, *others) -> None:
-    if not first.is_cuda:
+    dev = first.get_device()
+    if dev < 0:
         raise RuntimeError("clt_training_amd ops need tensors on an MI355X GPU (there is no CPU fallback)")
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
 
 
 def _call_on(t: Tensor, name: str, *args):
-    """``_call`` on the device of ``t`` and its current stream (appended), whatever the current device is."""
-    if t.device.index == torch.cuda.current_device():
-        _call(name, *args, _stream(t))
+    """``_call`` on the device of ``t`` and its current stream (appended), whatever the current device is.  (Pointers are
+    passed as integers and the stream is asked for as one: these calls are as short as a small kernel is.)"""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        _call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(t.device):
-            _call(name, *args, _stream(t))
+        with torch.cuda.device(dev):
+            _call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 class MXFP4Tensor:
@@ -674,22 +678,19 @@ class MXFP4Tensor:
     ``scales`` uint8 [rows, Kp / 32], with Kp = ``cols`` rounded up to a multiple of 128 (zero codes behind the last column).
     s = 255 marks a block that stands for NaN."""
 
-    __slots__ = ("codes", "scales", "cols")
+    __slots__ = ("codes", "scales", "cols", "shape")
 
     def __init__(self, codes: Tensor, scales: Tensor, cols: int):
         kp = -(-cols // 128) * 128
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
             raise TypeError("MXFP4Tensor: codes and scales are uint8 matrices")
-        if cols < 1 or codes.shape[1] != kp // 2 or scales.shape != (codes.shape[0], kp // 32):
+        rows = codes.size(0)
+        if cols < 1 or codes.size(1) != kp // 2 or scales.size(0) != rows or scales.size(1) != kp // 32:
             raise ValueError(f"MXFP4Tensor: {cols} columns need codes [rows, {kp // 2}] and scales [rows, {kp // 32}], "
                              f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.get_device() != scales.get_device():
             raise ValueError("MXFP4Tensor: codes and scales are contiguous and on one device")
-        self.codes, self.scales, self.cols = codes, scales, cols
-
-    @property
-    def shape(self):
-        return torch.Size((self.codes.shape[0], self.cols))
+        self.codes, self.scales, self.cols, self.shape = codes, scales, cols, torch.Size((rows, cols))
 
     @property
     def device(self):
@@ -702,8 +703,8 @@ class MXFP4Tensor:
         _same_device(self.codes)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         if out.numel():
-            _call_on(out, "clt_mxfp4_dequantize", _ptr(self.codes), _ptr(self.scales), self.shape[0], self.cols, _ptr(out),
-                     _DT[dtype])
+            _call_on(out, "clt_mxfp4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
+                     out.data_ptr(), _DT[dtype])
         return out
 
 
@@ -718,13 +719,14 @@ def mxfp4_quantize(x: Tensor) -> MXFP4Tensor:
     R, K = x.shape
     if K < 1:
         raise ValueError("mxfp4_quantize: no columns")
-    if K > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < 0:
+    if K > 1 and x.stride(1) != 1:
         x = x.contiguous()
     kp = -(-K // 128) * 128
     codes = torch.empty(R, kp // 2, dtype=torch.uint8, device=x.device)
     scales = torch.empty(R, kp // 32, dtype=torch.uint8, device=x.device)
     if R:
-        _call_on(x, "clt_mxfp4_quantize", _ptr(x), dt, x.stride(0) if R > 1 else K, R, K, _ptr(codes), _ptr(scales))
+        _call_on(x, "clt_mxfp4_quantize", x.data_ptr(), dt, x.stride(0) if R > 1 else K, R, K, codes.data_ptr(),
+                 scales.data_ptr())
     return MXFP4Tensor(codes, scales, K)
 
 
@@ -735,31 +737,45 @@ def mxfp4_linear(x, W: MXFP4Tensor, b: Optional[Tensor] = None, *, relu: bool = 
     dtype of ``x`` (float32 for an ``MXFP4Tensor``); ``out`` [N, M] may have any row stride."""
     if not isinstance(W, MXFP4Tensor):
         raise TypeError("mxfp4_linear: W is an MXFP4Tensor (mxfp4_quantize)")
+    packed = isinstance(x, MXFP4Tensor)
     if out_dtype is None:
-        out_dtype = out.dtype if out is not None else (torch.float32 if isinstance(x, MXFP4Tensor) else x.dtype)
+        out_dtype = out.dtype if out is not None else (torch.float32 if packed else x.dtype)
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}: only float32 / bfloat16")
-    if len(x.shape) != 2 or x.shape[1] != W.cols:
-        raise ValueError(f"mxfp4_linear: x {tuple(x.shape)} does not fit W {tuple(W.shape)}")
-    N, (M, K) = x.shape[0], W.shape
+    (M, K), shape = W.shape, x.shape
+    if len(shape) != 2 or shape[1] != K:
+        raise ValueError(f"mxfp4_linear: x {tuple(shape)} does not fit W {tuple(W.shape)}")
+    N = shape[0]
+    bp, bdt = None, 0
     if b is not None:
         if b.shape != (M,):
             raise ValueError(f"mxfp4_linear: bias {tuple(b.shape)} for {M} rows of W")
         b = _c(b)
-        bdt = _dt(b)
+        bp, bdt = b.data_ptr(), _dt(b)
+    codes = W.codes
+    if packed:
+        _same_device(codes, x.codes, b, out)
     else:
-        bdt = 0
-    _same_device(W.codes, x.codes if isinstance(x, MXFP4Tensor) else x, b, out)
+        xdt = _dt(x)
+        _same_device(codes, x, b, out)
     if out is None:
-        out = torch.empty(N, M, dtype=out_dtype, device=W.device)
+        out = torch.empty((N, M), dtype=out_dtype, device=codes.device)
     elif out.shape != (N, M) or out.dtype != out_dtype or M > 1 and out.stride(1) != 1 or N > 1 and out.stride(0) < M:
         raise ValueError(f"mxfp4_linear: out must be [{N}, {M}] {out_dtype} with rows that do not overlap")
     if N == 0 or M == 0:
         return out
-    if not isinstance(x, MXFP4Tensor):
-        x = mxfp4_quantize(x)
-    _call_on(out, "clt_mxfp4_linear", _ptr(x.codes), _ptr(x.scales), _ptr(W.codes), _ptr(W.scales), _ptr(b), bdt, N, M, K,
-             int(relu), _ptr(out), _DT[out_dtype], out.stride(0) if N > 1 else M)
+    tail = (codes.data_ptr(), W.scales.data_ptr(), bp, bdt, N, M, K, int(relu), out.data_ptr(), _DT[out_dtype],
+            out.stride(0) if N > 1 else M)
+    if packed:
+        _call_on(out, "clt_mxfp4_linear", x.codes.data_ptr(), x.scales.data_ptr(), *tail)
+        return out
+    if K > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    # (scratch from the allocator, not kept: a captured graph then holds its own)
+    nbytes = _lib.load().clt_mxfp4_linear_x_workspace_bytes(N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=codes.device) if nbytes else None
+    _call_on(out, "clt_mxfp4_linear_x", x.data_ptr(), xdt, x.stride(0) if N > 1 else K, *tail,
+             ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
@@ -774,9 +790,7 @@ def encode_topk_mxfp4(x: Tensor, W, b: Optional[Tensor], k: int, out_dtype=None,
     out_dtype = out_dtype or x.dtype
     if N == 0:
         return (torch.empty(0, k, dtype=out_dtype, device=x.device), torch.empty(0, k, dtype=torch.int64, device=x.device))
-    size = N * M * torch.empty((), dtype=out_dtype).element_size()
-    pre = workspace(x.device, size, "pre")[:size].view(out_dtype).view(N, M)
-    mxfp4_linear(x, W, b, relu=True, out=pre)
+    pre = mxfp4_linear(x, W, b, relu=True, out_dtype=out_dtype)
     return (topk_rows if activation == "topk" else groupmax_rows)(pre, k, out_dtype=out_dtype)
 
 
@@ -795,27 +809,28 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr=1e-3, beta
         raise ValueError("adamw_step: one gradient and two moments for every parameter")
     if n == 0:
         return
-    dev = params[0].device
     _same_device(params[0])
+    dev = params[0].get_device()
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step cannot be captured into a graph: the step count is a number of the call, and every "
                            "replay would repeat the same step")
-    lrs = lr if isinstance(lr, (list, tuple)) else None
-    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else None
-    if lrs is not None and len(lrs) != n or wds is not None and len(wds) != n:
+    lrs = lr if isinstance(lr, (list, tuple)) else [float(lr)] * n
+    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * n
+    if len(lrs) != n or len(wds) != n:
         raise ValueError("adamw_step: lr and weight_decay are numbers or one number per tensor")
-    one_lr, one_wd = (0.0 if lrs is not None else float(lr)), (0.0 if wds is not None else float(weight_decay))
-    table = (_lib.AdamWTensor * n)()
-    keep, seen, live = [], set(), 0  # (keep: the contiguous copies outlive the launch)
-    for i, (r, p, g, m, v) in enumerate(zip(table, params, grads, exp_avgs, exp_avg_sqs)):
-        if p.dtype not in _DT or g.dtype not in _DT:
+    pack = _ADAMW_RECORD.pack
+    table, keep, seen, live = [], [], set(), 0  # (keep: the contiguous copies outlive the launch)
+    for i, (p, g, m, v, one_lr, one_wd) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, lrs, wds)):
+        pdt, gdt = _DT.get(p.dtype), _DT.get(g.dtype)
+        if pdt is None or gdt is None:
             raise TypeError(f"adamw_step: tensor {i}: only float32 / bfloat16, got {p.dtype} and {g.dtype}")
-        if p.device != dev or g.device != dev or g.shape != p.shape or not p.is_contiguous():
-            raise ValueError(f"adamw_step: tensor {i}: a contiguous parameter and a gradient of its shape on {dev}")
+        if p.get_device() != dev or g.get_device() != dev or g.shape != p.shape or not p.is_contiguous():
+            raise ValueError(f"adamw_step: tensor {i}: a contiguous parameter and a gradient of its shape, on device {dev}")
         if not g.is_contiguous():
             g = g.contiguous()
             keep.append(g)
         numel = p.numel()
+        msp = vsp = 0
         if isinstance(m, (tuple, list)) != isinstance(v, (tuple, list)):
             raise ValueError(f"adamw_step: tensor {i}: both moments in 32 bits or both in 8")
         if isinstance(m, (tuple, list)):
@@ -825,28 +840,28 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr=1e-3, beta
                     raise TypeError(f"adamw_step: tensor {i}: 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
                                     f"float8_e8m0fnu scales, got {c.dtype} and {s.dtype}")
                 if (c.numel() != numel or s.numel() != -(-numel // 128) or not c.is_contiguous() or not s.is_contiguous()
-                        or c.device != dev or s.device != dev):
-                    raise ValueError(f"adamw_step: tensor {i}: one code per element and one scale per 128, contiguous, on {dev}")
-            r.m_scale, r.v_scale = ms.data_ptr() or None, vs.data_ptr() or None
+                        or c.get_device() != dev or s.get_device() != dev):
+                    raise ValueError(f"adamw_step: tensor {i}: one code per element and one scale per 128, contiguous, on "
+                                     f"device {dev}")
+            msp, vsp = ms.data_ptr(), vs.data_ptr()
         else:
             for c in (m, v):
                 if c.dtype != torch.float32:
                     raise TypeError(f"adamw_step: tensor {i}: moments are float32 or 8-bit pairs, got {c.dtype}")
-                if c.shape != p.shape or not c.is_contiguous() or c.device != dev:
-                    raise ValueError(f"adamw_step: tensor {i}: moments of the parameter's shape, contiguous, on {dev}")
-        r.p, r.g, r.m, r.v = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
-        r.numel = numel
+                if c.shape != p.shape or not c.is_contiguous() or c.get_device() != dev:
+                    raise ValueError(f"adamw_step: tensor {i}: moments of the parameter's shape, contiguous, on device {dev}")
+        pp, mp, vp = p.data_ptr(), m.data_ptr(), v.data_ptr()
         if numel:
             live += 1
-            seen.update((r.p, r.m, r.v))
-        r.lr = one_lr if lrs is None else float(lrs[i])
-        r.weight_decay = one_wd if wds is None else float(wds[i])
-        r.p_dtype, r.g_dtype = _DT[p.dtype], _DT[g.dtype]
+            seen.update((pp, mp, vp))
+        table.append(pack(pp, g.data_ptr(), mp, vp, msp, vsp, numel, one_lr, one_wd, pdt, gdt))
     if len(seen) != 3 * live:
         raise ValueError("adamw_step: a tensor is given twice (parameters and moments are updated in place)")
-    _call_on(params[0], "clt_adamw_step", C.cast(table, C.c_void_p), n, float(betas[0]), float(betas[1]), float(eps),
-             int(step), int(seed) & 0xFFFFFFFF)
+    _call_on(params[0], "clt_adamw_step", b"".join(table), n, float(betas[0]), float(betas[1]), float(eps), int(step),
+             int(seed) & 0xFFFFFFFF)
 
 
+_ADAMW_RECORD = struct.Struct("6Qq2d2i")  # clt_adamw_tensor
+assert _ADAMW_RECORD.size == C.sizeof(_lib.AdamWTensor)
 _CODES8 = (torch.uint8, torch.float8_e4m3fn)
 _SCALES8 = (torch.uint8, torch.float8_e8m0fnu)

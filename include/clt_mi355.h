@@ -438,6 +438,14 @@ int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint
                      const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K, int relu, void* out, int out_dtype,
                      int64_t ldo, clt_stream_t stream);
 
+/* quantize and linear in one call, for x [N, K] `x_dtype` with rows ldx elements apart: the codes of x go through
+ * `workspace` (clt_mxfp4_linear_x_workspace_bytes(N, K) bytes, 16-byte aligned, nothing in it outlives the call), or, for
+ * few tokens (0 bytes needed), are made inside the product's launch.  The same results as the two calls. */
+size_t clt_mxfp4_linear_x_workspace_bytes(int64_t N, int64_t K);
+int clt_mxfp4_linear_x(const void* x, int x_dtype, int64_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
+                       const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K, int relu, void* out, int out_dtype,
+                       int64_t ldo, void* workspace, size_t workspace_bytes, clt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
