@@ -135,6 +135,28 @@ def load():
     return lib
 
 
+_host = None
+
+
+def host():
+    """The compiled host side of the short calls (csrc/host.cpp), bound to this library's functions; raises when it is not
+    built (no fallback)."""
+    global _host
+    if _host is None:
+        lib = load()
+        import torch  # noqa: F401 (the module links against it)
+        try:
+            from . import _clthost
+        except ImportError as e:
+            raise RuntimeError(f"{HERE / '_clthost.so'} not found or not loadable ({e}). "
+                               "Build it with `python -m clt_training_amd.build`.") from None
+        _clthost.bind({name: C.cast(getattr(lib, name), _vp).value for name in
+                       ("clt_last_error", "clt_mxfp4_quantize", "clt_mxfp4_dequantize", "clt_mxfp4_linear",
+                        "clt_mxfp4_linear_x", "clt_mxfp4_linear_x_workspace_bytes", "clt_adamw_step")})
+        _host = _clthost
+    return _host
+
+
 CLT_ERR_UNSUPPORTED = -2  # (include/clt_mi355.h)
 
 

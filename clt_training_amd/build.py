@@ -18,6 +18,24 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-res
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+# The compiled host side (csrc/host.cpp): a Python module against this process's torch, built by the host compiler.
+HOST_LIB = HERE / "_clthost.so"
+
+
+def _host_command(out: Path) -> list:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    includes = [*include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(a for p in includes for a in ("-isystem", str(p))), str(CSRC / "host.cpp"), "-o", str(out), f"-L{lib}",
+            "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"]
+
+
 def _stale(out: Path, deps) -> bool:
     if not out.exists():
         return True
@@ -43,8 +61,17 @@ def build(force: bool = False, verbose: bool = True, tuning: bool = False) -> Pa
             subprocess.run(cmd, check=True)
         return obj
 
-    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+    def compile_host():
+        if force or _stale(HOST_LIB, [CSRC / "host.cpp", HERE.parent / "include" / "clt_mi355.h"]):
+            cmd = _host_command(HOST_LIB)
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True)
+
+    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 1)) as ex:
+        host = ex.submit(compile_host)
         objs = list(ex.map(compile_one, SOURCES))
+        host.result()
     if force or _stale(lib, objs):
         cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(lib), *map(str, objs)]
         if verbose:

@@ -1,0 +1,266 @@
+// Host side of the short calls: argument checks, allocation and launch of the MXFP4 and AdamW entry points of libcltmi355.so
+// for torch tensors.  What a kernel of a few microseconds costs from Python is mostly this, so it is compiled; the library's
+// functions are handed over as addresses (bind), so that there is one loader (_lib.py) and one library.
+#include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/utils/pybind.h>
+#include <torch/extension.h>
+
+#include <string>
+#include <unordered_set>
+#include <vector>
+
+#include "../../include/clt_mi355.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+namespace {
+
+decltype(&clt_last_error) last_error = nullptr;
+decltype(&clt_mxfp4_quantize) quantize_fn = nullptr;
+decltype(&clt_mxfp4_dequantize) dequantize_fn = nullptr;
+decltype(&clt_mxfp4_linear) linear_fn = nullptr;
+decltype(&clt_mxfp4_linear_x) linear_x_fn = nullptr;
+decltype(&clt_mxfp4_linear_x_workspace_bytes) linear_x_bytes_fn = nullptr;
+decltype(&clt_adamw_step) adamw_fn = nullptr;
+
+void bind(const py::dict& address) {
+  auto take = [&](auto& fn, const char* name) {
+    fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(address[name].cast<uintptr_t>());
+  };
+  take(last_error, "clt_last_error");
+  take(quantize_fn, "clt_mxfp4_quantize");
+  take(dequantize_fn, "clt_mxfp4_dequantize");
+  take(linear_fn, "clt_mxfp4_linear");
+  take(linear_x_fn, "clt_mxfp4_linear_x");
+  take(linear_x_bytes_fn, "clt_mxfp4_linear_x_workspace_bytes");
+  take(adamw_fn, "clt_adamw_step");
+}
+
+void check(int rc, const char* name) {
+  TORCH_CHECK(rc == 0, name, " failed (status ", rc, "): ", last_error());
+}
+
+int code_of(at::ScalarType t) {
+  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16, "unsupported dtype ", t, ": only float32 / bfloat16");
+  return t == at::kFloat ? CLT_F32 : CLT_BF16;
+}
+void on_gpu(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "clt_training_amd ops need tensors on an MI355X GPU (there is no CPU fallback)");
+}
+void same_device(const Tensor& a, const Tensor& b) {
+  TORCH_CHECK_VALUE(a.device() == b.device(), "tensors on different devices: ", a.device(), " and ", b.device());
+}
+int64_t padded(int64_t K) { return (K + 127) / 128 * 128; }
+
+// the device of `t` for the calls below, and its current stream
+struct On {
+  c10::DeviceIndex before, now;
+  void* stream;
+  explicit On(const Tensor& t) : before(c10::hip::current_device()), now(t.device().index()) {
+    if (now != before) c10::hip::set_device(now);
+    stream = c10::hip::getCurrentHIPStream(now).stream();
+  }
+  ~On() {
+    if (now != before) c10::hip::set_device(before);
+  }
+};
+
+// rows of unit stride (a copy if they have another)
+Tensor rows_of(const Tensor& x) { return x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x; }
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+void check_codes(const Tensor& codes, const Tensor& scales, int64_t cols) {
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.dim() == 2 && scales.dim() == 2,
+                   "MXFP4Tensor: codes and scales are uint8 matrices");
+  const int64_t kp = padded(cols);
+  TORCH_CHECK_VALUE(cols >= 1 && codes.size(1) == kp / 2 && scales.size(0) == codes.size(0) && scales.size(1) == kp / 32,
+                    "MXFP4Tensor: ", cols, " columns need codes [rows, ", kp / 2, "] and scales [rows, ", kp / 32, "], got ",
+                    codes.sizes(), " and ", scales.sizes());
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous() && codes.device() == scales.device(),
+                    "MXFP4Tensor: codes and scales are contiguous and on one device");
+}
+
+std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x_) {
+  TORCH_CHECK_VALUE(x_.dim() == 2, "mxfp4_quantize: a matrix is needed, got shape ", x_.sizes());
+  const int dt = code_of(x_.scalar_type());
+  on_gpu(x_);
+  TORCH_CHECK_VALUE(x_.size(1) >= 1, "mxfp4_quantize: no columns");
+  const Tensor x = rows_of(x_);
+  const int64_t R = x.size(0), K = x.size(1), kp = padded(K);
+  const auto opt = x.options().dtype(at::kByte);
+  Tensor codes = at::empty({R, kp / 2}, opt), scales = at::empty({R, kp / 32}, opt);
+  if (R) {
+    const On on(x);
+    check(quantize_fn(x.const_data_ptr(), dt, row_stride(x), R, K, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+                      on.stream),
+          "clt_mxfp4_quantize");
+  }
+  return {codes, scales};
+}
+
+Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, at::ScalarType dtype) {
+  const int dt = code_of(dtype);
+  on_gpu(codes);
+  check_codes(codes, scales, cols);
+  Tensor out = at::empty({codes.size(0), cols}, codes.options().dtype(dtype));
+  if (out.numel()) {
+    const On on(out);
+    check(dequantize_fn(codes.const_data_ptr<uint8_t>(), scales.const_data_ptr<uint8_t>(), codes.size(0), cols,
+                        out.mutable_data_ptr(), dt, on.stream),
+          "clt_mxfp4_dequantize");
+  }
+  return out;
+}
+
+// x: a matrix, or codes with their scales
+Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& codes, const Tensor& scales, int64_t cols,
+                    const OptTensor& bias_, bool relu, std::optional<at::ScalarType> dtype, const OptTensor& out_) {
+  const bool packed = x_scales.has_value();
+  const auto odt = dtype ? *dtype : out_ ? out_->scalar_type() : packed ? at::kFloat : x_.scalar_type();
+  const int oc = code_of(odt);
+  check_codes(codes, scales, cols);
+  if (packed) check_codes(x_, *x_scales, cols);
+  TORCH_CHECK_VALUE(x_.dim() == 2 && (packed || x_.size(1) == cols), "mxfp4_linear: x ", x_.sizes(), " does not fit W [",
+                    codes.size(0), ", ", cols, "]");
+  const int64_t N = x_.size(0), M = codes.size(0);
+  Tensor bias;
+  int bc = 0;
+  if (bias_) {
+    TORCH_CHECK_VALUE(bias_->dim() == 1 && bias_->size(0) == M, "mxfp4_linear: bias ", bias_->sizes(), " for ", M, " rows of W");
+    bc = code_of(bias_->scalar_type());
+    bias = bias_->contiguous();
+  }
+  const int xc = packed ? 0 : code_of(x_.scalar_type());
+  on_gpu(codes);
+  same_device(codes, x_);
+  if (bias_) same_device(codes, bias);
+  Tensor out;
+  if (out_) {
+    out = *out_;
+    same_device(codes, out);
+    TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == N && out.size(1) == M && out.scalar_type() == odt &&
+                          (M <= 1 || out.stride(1) == 1) && (N <= 1 || out.stride(0) >= M),
+                      "mxfp4_linear: out must be [", N, ", ", M, "] ", odt, " with rows that do not overlap");
+  } else {
+    out = at::empty({N, M}, codes.options().dtype(odt));
+  }
+  if (N == 0 || M == 0) return out;
+  const On on(out);
+  const int64_t ldo = N > 1 ? out.stride(0) : M;
+  const uint8_t *wc = codes.const_data_ptr<uint8_t>(), *ws = scales.const_data_ptr<uint8_t>();
+  const void* bp = bias_ ? bias.const_data_ptr() : nullptr;
+  if (packed) {
+    check(linear_fn(x_.const_data_ptr<uint8_t>(), x_scales->const_data_ptr<uint8_t>(), wc, ws, bp, bc, N, M, cols, relu,
+                    out.mutable_data_ptr(), oc, ldo, on.stream),
+          "clt_mxfp4_linear");
+    return out;
+  }
+  const Tensor x = rows_of(x_);
+  const size_t bytes = linear_x_bytes_fn(N, cols);
+  Tensor scratch;  // (from the allocator, not kept: a captured graph then holds its own)
+  if (bytes) scratch = at::empty({(int64_t)bytes}, codes.options());
+  check(linear_x_fn(x.const_data_ptr(), xc, row_stride(x), wc, ws, bp, bc, N, M, cols, relu, out.mutable_data_ptr(), oc, ldo,
+                    bytes ? scratch.data_ptr() : nullptr, bytes, on.stream),
+        "clt_mxfp4_linear_x");
+  return out;
+}
+
+// a number, or one per tensor
+std::vector<double> per_tensor(const py::object& v, size_t n, const char* name) {
+  if (py::isinstance<py::list>(v) || py::isinstance<py::tuple>(v)) {
+    auto r = v.cast<std::vector<double>>();
+    TORCH_CHECK_VALUE(r.size() == n, "adamw_step: ", name, " is a number or one number per tensor");
+    return r;
+  }
+  return std::vector<double>(n, v.cast<double>());
+}
+
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const py::sequence& first,
+                const py::sequence& second, int64_t step, const py::object& lr, std::pair<double, double> betas, double eps,
+                const py::object& weight_decay, int64_t seed) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && first.size() == n && second.size() == n,
+                    "adamw_step: one gradient and two moments for every parameter");
+  if (!n) return;
+  on_gpu(params[0]);
+  const auto dev = params[0].device();
+  const auto lrs = per_tensor(lr, n, "lr"), wds = per_tensor(weight_decay, n, "weight_decay");
+  const On on(params[0]);
+  {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing((hipStream_t)on.stream, &status) == hipSuccess, "adamw_step: stream state");
+    TORCH_CHECK(status == hipStreamCaptureStatusNone, "adamw_step cannot be captured into a graph: the step count is a number "
+                "of the call, and every replay would repeat the same step");
+  }
+  std::vector<clt_adamw_tensor> table(n);
+  std::vector<Tensor> keep;  // contiguous copies outlive the launch, and so do the moments
+  std::unordered_set<const void*> seen;
+  size_t live = 0;
+  keep.reserve(4 * n);
+  seen.reserve(6 * n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    Tensor g = grads[i];
+    clt_adamw_tensor& r = table[i];
+    r = {};
+    TORCH_CHECK_TYPE((p.scalar_type() == at::kFloat || p.scalar_type() == at::kBFloat16) &&
+                         (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),
+                     "adamw_step: tensor ", i, ": only float32 / bfloat16, got ", p.scalar_type(), " and ", g.scalar_type());
+    TORCH_CHECK_VALUE(p.device() == dev && g.device() == dev && g.sizes() == p.sizes() && p.is_contiguous(),
+                      "adamw_step: tensor ", i, ": a contiguous parameter and a gradient of its shape, on ", dev);
+    if (!g.is_contiguous()) keep.push_back(g = g.contiguous());
+    const int64_t numel = p.numel();
+    const py::object fo = first[i], so = second[i];
+    const bool eight = !THPVariable_Check(fo.ptr());
+    TORCH_CHECK_VALUE(eight != THPVariable_Check(so.ptr()), "adamw_step: tensor ", i, ": both moments in 32 bits or both in 8");
+    void* ptr[2];
+    for (int k = 0; k < 2; ++k) {
+      const py::object& o = k ? so : fo;
+      if (!eight) {
+        const Tensor& c = THPVariable_Unpack(o.ptr());
+        TORCH_CHECK_TYPE(c.scalar_type() == at::kFloat, "adamw_step: tensor ", i, ": moments are float32 or 8-bit pairs, got ",
+                         c.scalar_type());
+        TORCH_CHECK_VALUE(c.sizes() == p.sizes() && c.is_contiguous() && c.device() == dev, "adamw_step: tensor ", i,
+                          ": moments of the parameter's shape, contiguous, on ", dev);
+        ptr[k] = c.mutable_data_ptr();
+      } else {
+        const auto pair = o.cast<std::pair<Tensor, Tensor>>();
+        const auto ct = pair.first.scalar_type(), st = pair.second.scalar_type();
+        TORCH_CHECK_TYPE((ct == at::kByte || ct == at::kFloat8_e4m3fn) && (st == at::kByte || st == at::kFloat8_e8m0fnu),
+                         "adamw_step: tensor ", i, ": 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
+                         "float8_e8m0fnu scales, got ", ct, " and ", st);
+        TORCH_CHECK_VALUE(pair.first.numel() == numel && pair.second.numel() == (numel + 127) / 128 &&
+                              pair.first.is_contiguous() && pair.second.is_contiguous() && pair.first.device() == dev &&
+                              pair.second.device() == dev,
+                          "adamw_step: tensor ", i, ": one code per element and one scale per 128, contiguous, on ", dev);
+        ptr[k] = pair.first.mutable_data_ptr();
+        (k ? r.v_scale : r.m_scale) = static_cast<uint8_t*>(pair.second.mutable_data_ptr());
+      }
+    }
+    r.p = p.mutable_data_ptr(), r.g = g.const_data_ptr(), r.m = ptr[0], r.v = ptr[1];
+    r.numel = numel, r.lr = lrs[i], r.weight_decay = wds[i];
+    r.p_dtype = p.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
+    r.g_dtype = g.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
+    if (numel) {
+      ++live;
+      seen.insert(r.p), seen.insert(r.m), seen.insert(r.v);
+    }
+  }
+  TORCH_CHECK_VALUE(seen.size() == 3 * live, "adamw_step: a tensor is given twice (parameters and moments are updated in place)");
+  check(adamw_fn(table.data(), (int)n, betas.first, betas.second, eps, step, (uint32_t)seed, on.stream), "clt_adamw_step");
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_clthost, m) {
+  m.def("bind", &bind);
+  m.def("check_codes", &check_codes);
+  m.def("mxfp4_quantize", &mxfp4_quantize);
+  m.def("mxfp4_dequantize", &mxfp4_dequantize);
+  m.def("mxfp4_linear", &mxfp4_linear);
+  m.def("adamw_step", &adamw_step);
+}

@@ -6,7 +6,6 @@ if the tensors are not on a GPU."""
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from typing import Optional
 
 import torch
@@ -652,24 +651,18 @@ def fvu_grad(y: Tensor, yhat: Tensor, mask: Optional[Tensor], l2tv: Tensor, gsca
 
 
 # ----------------------------------------------------------------------------- MXFP4: 4-bit microscaled encoder
-def _same_device(first: Tensor, *others) -> None:
-    dev = first.get_device()
-    if dev < 0:
-        raise RuntimeError("clt_training_amd ops need tensors on an MI355X GPU (there is no CPU fallback)")
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
-
-
-def _call_on(t: Tensor, name: str, *args):
-    """``_call`` on the device of ``t`` and its current stream (appended), whatever the current device is.  (Pointers are
-    passed as integers and the stream is asked for as one: these calls are as short as a small kernel is.)"""
-    dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        _call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            _call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+def _host_call(name: str, fn: str, *args):
+    """A call of the compiled host side (csrc/host.cpp: checks, allocation, device, stream, launch), timed like ``_call``."""
+    f = getattr(_lib.host(), fn)
+    prof = PROFILE
+    if prof is None or not prof.active or not (prof.names is None or name in prof.names):
+        return f(*args)
+    s, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    s.record()
+    out = f(*args)
+    e.record()
+    prof.add(name, s, e)
+    return out
 
 
 class MXFP4Tensor:
@@ -678,19 +671,15 @@ class MXFP4Tensor:
     ``scales`` uint8 [rows, Kp / 32], with Kp = ``cols`` rounded up to a multiple of 128 (zero codes behind the last column).
     s = 255 marks a block that stands for NaN."""
 
-    __slots__ = ("codes", "scales", "cols", "shape")
+    __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes: Tensor, scales: Tensor, cols: int):
-        kp = -(-cols // 128) * 128
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
-            raise TypeError("MXFP4Tensor: codes and scales are uint8 matrices")
-        rows = codes.size(0)
-        if cols < 1 or codes.size(1) != kp // 2 or scales.size(0) != rows or scales.size(1) != kp // 32:
-            raise ValueError(f"MXFP4Tensor: {cols} columns need codes [rows, {kp // 2}] and scales [rows, {kp // 32}], "
-                             f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.get_device() != scales.get_device():
-            raise ValueError("MXFP4Tensor: codes and scales are contiguous and on one device")
-        self.codes, self.scales, self.cols, self.shape = codes, scales, cols, torch.Size((rows, cols))
+        _lib.host().check_codes(codes, scales, cols)
+        self.codes, self.scales, self.cols = codes, scales, cols
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.cols))
 
     @property
     def device(self):
@@ -698,36 +687,17 @@ class MXFP4Tensor:
 
     def dequantize(self, dtype=torch.float32) -> Tensor:
         """The values, [rows, cols] (bfloat16 holds each of them exactly)."""
-        if dtype not in _DT:
-            raise TypeError(f"unsupported dtype {dtype}: only float32 / bfloat16")
-        _same_device(self.codes)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        if out.numel():
-            _call_on(out, "clt_mxfp4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.cols,
-                     out.data_ptr(), _DT[dtype])
-        return out
+        return _host_call("clt_mxfp4_dequantize", "mxfp4_dequantize", self.codes, self.scales, self.cols, dtype)
 
 
 def mxfp4_quantize(x: Tensor) -> MXFP4Tensor:
-    """Rows of ``x`` [R, K] (float32 / bfloat16, unit stride along K) to MXFP4: the scale of a block of 32 is
+    """Rows of ``x`` [R, K] (float32 / bfloat16, any strides) to MXFP4: the scale of a block of 32 is
     2^(floor(log2 max |x|) - 2), values are rounded to nearest even and saturate at 6; a block with a NaN or an infinity
     becomes NaN."""
-    if x.dim() != 2:
-        raise ValueError(f"mxfp4_quantize: a matrix is needed, got shape {tuple(x.shape)}")
-    dt = _dt(x)
-    _same_device(x)
-    R, K = x.shape
-    if K < 1:
-        raise ValueError("mxfp4_quantize: no columns")
-    if K > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    kp = -(-K // 128) * 128
-    codes = torch.empty(R, kp // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(R, kp // 32, dtype=torch.uint8, device=x.device)
-    if R:
-        _call_on(x, "clt_mxfp4_quantize", x.data_ptr(), dt, x.stride(0) if R > 1 else K, R, K, codes.data_ptr(),
-                 scales.data_ptr())
-    return MXFP4Tensor(codes, scales, K)
+    q = MXFP4Tensor.__new__(MXFP4Tensor)
+    q.codes, q.scales = _host_call("clt_mxfp4_quantize", "mxfp4_quantize", x)
+    q.cols = x.shape[1]
+    return q
 
 
 def mxfp4_linear(x, W: MXFP4Tensor, b: Optional[Tensor] = None, *, relu: bool = False, out_dtype=None,
@@ -737,46 +707,12 @@ def mxfp4_linear(x, W: MXFP4Tensor, b: Optional[Tensor] = None, *, relu: bool = 
     dtype of ``x`` (float32 for an ``MXFP4Tensor``); ``out`` [N, M] may have any row stride."""
     if not isinstance(W, MXFP4Tensor):
         raise TypeError("mxfp4_linear: W is an MXFP4Tensor (mxfp4_quantize)")
-    packed = isinstance(x, MXFP4Tensor)
-    if out_dtype is None:
-        out_dtype = out.dtype if out is not None else (torch.float32 if packed else x.dtype)
-    if out_dtype not in _DT:
-        raise TypeError(f"unsupported dtype {out_dtype}: only float32 / bfloat16")
-    (M, K), shape = W.shape, x.shape
-    if len(shape) != 2 or shape[1] != K:
-        raise ValueError(f"mxfp4_linear: x {tuple(shape)} does not fit W {tuple(W.shape)}")
-    N = shape[0]
-    bp, bdt = None, 0
-    if b is not None:
-        if b.shape != (M,):
-            raise ValueError(f"mxfp4_linear: bias {tuple(b.shape)} for {M} rows of W")
-        b = _c(b)
-        bp, bdt = b.data_ptr(), _dt(b)
-    codes = W.codes
-    if packed:
-        _same_device(codes, x.codes, b, out)
-    else:
-        xdt = _dt(x)
-        _same_device(codes, x, b, out)
-    if out is None:
-        out = torch.empty((N, M), dtype=out_dtype, device=codes.device)
-    elif out.shape != (N, M) or out.dtype != out_dtype or M > 1 and out.stride(1) != 1 or N > 1 and out.stride(0) < M:
-        raise ValueError(f"mxfp4_linear: out must be [{N}, {M}] {out_dtype} with rows that do not overlap")
-    if N == 0 or M == 0:
-        return out
-    tail = (codes.data_ptr(), W.scales.data_ptr(), bp, bdt, N, M, K, int(relu), out.data_ptr(), _DT[out_dtype],
-            out.stride(0) if N > 1 else M)
-    if packed:
-        _call_on(out, "clt_mxfp4_linear", x.codes.data_ptr(), x.scales.data_ptr(), *tail)
-        return out
-    if K > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    # (scratch from the allocator, not kept: a captured graph then holds its own)
-    nbytes = _lib.load().clt_mxfp4_linear_x_workspace_bytes(N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=codes.device) if nbytes else None
-    _call_on(out, "clt_mxfp4_linear_x", x.data_ptr(), xdt, x.stride(0) if N > 1 else K, *tail,
-             ws.data_ptr() if nbytes else None, nbytes)
-    return out
+    if isinstance(x, MXFP4Tensor):
+        if x.cols != W.cols:
+            raise ValueError(f"mxfp4_linear: x {tuple(x.shape)} does not fit W {tuple(W.shape)}")
+        return _host_call("clt_mxfp4_linear", "mxfp4_linear", x.codes, x.scales, W.codes, W.scales, W.cols, b, relu, out_dtype,
+                          out)
+    return _host_call("clt_mxfp4_linear_x", "mxfp4_linear", x, None, W.codes, W.scales, W.cols, b, relu, out_dtype, out)
 
 
 def encode_topk_mxfp4(x: Tensor, W, b: Optional[Tensor], k: int, out_dtype=None, activation: str = "topk"):
@@ -804,64 +740,4 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr=1e-3, beta
     first moment and the SQUARE ROOT of the second in e4m3 times a power of two (all zero bytes: zero moments), rounded
     stochastically with random bits that ``seed``, the position in the list, ``step`` and the element determine.
     ``lr`` and ``weight_decay`` are numbers or one number per tensor; ``step`` counts from 1."""
-    n = len(params)
-    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n):
-        raise ValueError("adamw_step: one gradient and two moments for every parameter")
-    if n == 0:
-        return
-    _same_device(params[0])
-    dev = params[0].get_device()
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step cannot be captured into a graph: the step count is a number of the call, and every "
-                           "replay would repeat the same step")
-    lrs = lr if isinstance(lr, (list, tuple)) else [float(lr)] * n
-    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * n
-    if len(lrs) != n or len(wds) != n:
-        raise ValueError("adamw_step: lr and weight_decay are numbers or one number per tensor")
-    pack = _ADAMW_RECORD.pack
-    table, keep, seen, live = [], [], set(), 0  # (keep: the contiguous copies outlive the launch)
-    for i, (p, g, m, v, one_lr, one_wd) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, lrs, wds)):
-        pdt, gdt = _DT.get(p.dtype), _DT.get(g.dtype)
-        if pdt is None or gdt is None:
-            raise TypeError(f"adamw_step: tensor {i}: only float32 / bfloat16, got {p.dtype} and {g.dtype}")
-        if p.get_device() != dev or g.get_device() != dev or g.shape != p.shape or not p.is_contiguous():
-            raise ValueError(f"adamw_step: tensor {i}: a contiguous parameter and a gradient of its shape, on device {dev}")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            keep.append(g)
-        numel = p.numel()
-        msp = vsp = 0
-        if isinstance(m, (tuple, list)) != isinstance(v, (tuple, list)):
-            raise ValueError(f"adamw_step: tensor {i}: both moments in 32 bits or both in 8")
-        if isinstance(m, (tuple, list)):
-            (m, ms), (v, vs) = m, v
-            for c, s in ((m, ms), (v, vs)):
-                if c.dtype not in _CODES8 or s.dtype not in _SCALES8:
-                    raise TypeError(f"adamw_step: tensor {i}: 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
-                                    f"float8_e8m0fnu scales, got {c.dtype} and {s.dtype}")
-                if (c.numel() != numel or s.numel() != -(-numel // 128) or not c.is_contiguous() or not s.is_contiguous()
-                        or c.get_device() != dev or s.get_device() != dev):
-                    raise ValueError(f"adamw_step: tensor {i}: one code per element and one scale per 128, contiguous, on "
-                                     f"device {dev}")
-            msp, vsp = ms.data_ptr(), vs.data_ptr()
-        else:
-            for c in (m, v):
-                if c.dtype != torch.float32:
-                    raise TypeError(f"adamw_step: tensor {i}: moments are float32 or 8-bit pairs, got {c.dtype}")
-                if c.shape != p.shape or not c.is_contiguous() or c.get_device() != dev:
-                    raise ValueError(f"adamw_step: tensor {i}: moments of the parameter's shape, contiguous, on device {dev}")
-        pp, mp, vp = p.data_ptr(), m.data_ptr(), v.data_ptr()
-        if numel:
-            live += 1
-            seen.update((pp, mp, vp))
-        table.append(pack(pp, g.data_ptr(), mp, vp, msp, vsp, numel, one_lr, one_wd, pdt, gdt))
-    if len(seen) != 3 * live:
-        raise ValueError("adamw_step: a tensor is given twice (parameters and moments are updated in place)")
-    _call_on(params[0], "clt_adamw_step", b"".join(table), n, float(betas[0]), float(betas[1]), float(eps), int(step),
-             int(seed) & 0xFFFFFFFF)
-
-
-_ADAMW_RECORD = struct.Struct("6Qq2d2i")  # clt_adamw_tensor
-assert _ADAMW_RECORD.size == C.sizeof(_lib.AdamWTensor)
-_CODES8 = (torch.uint8, torch.float8_e4m3fn)
-_SCALES8 = (torch.uint8, torch.float8_e8m0fnu)
+    _host_call("clt_adamw_step", "adamw_step", params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, seed)
