@@ -4,7 +4,9 @@
 //   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // HBM-bound: per element 2 sizeof(p) + sizeof(g) bytes of parameter and gradient plus 16 (fp32 moments) or 4 + 4/128 (8-bit
-// moments).  One launch takes up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device
+// moments).  Measured on four 98304 x 768 bf16 tables with bf16 gradients: 1.22 ms, 5.45 TB/s (fp32 moments), 0.53 ms, 5.7 TB/s
+// (8-bit moments); a large copy reaches 4.9 TB/s here.  The 8-bit path is near the vector units' limit, too: with the
+// stochastic rounding written out in integer arithmetic instead of the hardware's conversion it took 0.61 ms.  One launch takes up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device
 // memory, so nothing is uploaded, kept between calls or shared by two streams.  A workgroup owns one chunk of one tensor.
 //
 // 8-bit moments.  m and r = sqrt(v) are e4m3 (v itself spans twice the binades: a factor 2^17.8 between the largest and
@@ -23,7 +25,7 @@ namespace {
 
 constexpr int MAX_TENSORS = 40;   // records in one launch's arguments (40 x 88 bytes: the argument segment holds 4 KiB)
 constexpr int VEC = 8;            // elements per lane and pass
-constexpr int PASS = 256 * VEC;   // elements per workgroup and pass
+constexpr int CHUNK = 256 * VEC;  // elements per workgroup (twice as many: +3 %, four times: +9 % on 302 M elements)
 constexpr int BLOCK8 = 128;       // elements per scale
 
 struct Rec {
@@ -44,7 +46,6 @@ struct Rec {
 struct Args {
   Rec rec[MAX_TENSORS];
   int n;
-  int chunk_elems;
   float c1, b2, c2, inv_sqrt_bc2, eps;  // 1 - b1, b2, 1 - b2
 };
 static_assert(sizeof(Args) <= 4096, "kernel arguments");
@@ -55,16 +56,58 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {  // two rounds 
   return x ^ (x >> 15);
 }
 
-// Eight elements from an address with no more than the element's own alignment (gfx950 takes dword loads at any byte).
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Eight elements from an address with no more than the element's own alignment (gfx950 takes dword loads at any byte), each
+// read and written once.  (Non-temporal stores, plain loads: 5.47 and 4.87 TB/s with fp32 and 8-bit moments of bf16 tables; both
+// non-temporal 5.29 and 4.95, loads only 5.19 and 4.77, neither 5.48 and 4.80.)
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Raw8 {
+struct Vec8;
+template <>
+struct Vec8<float> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+  static constexpr int N = 2;
+};
+template <>
+struct Vec8<bf16_t> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+  static constexpr int N = 1;
+};
+template <>
+struct Vec8<uint8_t> {
+  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(1)));
+  static constexpr int N = 1;
+};
+template <typename T>
+struct Raw8 {
   T e[8];
 };
+template <typename T>
+__device__ __forceinline__ Raw8<T> read8(const void* p) {
+  typedef typename Vec8<T>::type V;
+  constexpr int N = Vec8<T>::N;
+  V v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const V*>(p)[i];
+  Raw8<T> r;
+  __builtin_memcpy(&r, v, sizeof(r));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void write8(void* p, const Raw8<T>& r) {
+  typedef typename Vec8<T>::type V;
+  constexpr int N = Vec8<T>::N;
+  V v[N];
+  __builtin_memcpy(v, &r, sizeof(r));
+#pragma unroll
+  for (int i = 0; i < N; ++i) __builtin_nontemporal_store(v[i], reinterpret_cast<V*>(p) + i);
+}
 template <typename T>
 __device__ __forceinline__ void load8(const char* base, int64_t i, int n, float (&f)[8]) {
   const T* p = reinterpret_cast<const T*>(base) + i;
   if (n >= 8) {
-    const Raw8<T> r = *reinterpret_cast<const Raw8<T>*>(p);
+    const Raw8<T> r = read8<T>(p);
 #pragma unroll
     for (int q = 0; q < 8; ++q) f[q] = (float)r.e[q];
   } else {
@@ -77,9 +120,16 @@ __device__ __forceinline__ void store8(char* base, int64_t i, int n, const float
   T* p = reinterpret_cast<T*>(base) + i;
   if (n >= 8) {
     Raw8<T> r;
+    if constexpr (sizeof(T) == 2) {  // (in pairs: one v_cvt_pk_bf16_f32)
+      bf16x2 w[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) r.e[q] = (T)f[q];
-    *reinterpret_cast<Raw8<T>*>(p) = r;
+      for (int q = 0; q < 4; ++q) w[q] = __builtin_convertvector(f32x2{f[2 * q], f[2 * q + 1]}, bf16x2);
+      __builtin_memcpy(&r, w, sizeof(r));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) r.e[q] = (T)f[q];
+    }
+    write8<T>(p, r);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -87,13 +137,11 @@ __device__ __forceinline__ void store8(char* base, int64_t i, int n, const float
   }
 }
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
 // eight e4m3 codes
 __device__ __forceinline__ void load_codes(const char* base, int64_t i, int n, float scale, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
   if (n >= 8) {
-    const Raw8<uint8_t> r = *reinterpret_cast<const Raw8<uint8_t>*>(base + i);
+    const Raw8<uint8_t> r = read8<uint8_t>(base + i);
     __builtin_memcpy(w, &r, 8);
   } else {
     for (int q = 0; q < n; ++q) w[q >> 2] |= (uint32_t)(uint8_t)base[i + q] << (8 * (q & 3));
@@ -105,118 +153,115 @@ __device__ __forceinline__ void load_codes(const char* base, int64_t i, int n, f
     f[4 * h] = a.x * scale, f[4 * h + 1] = a.y * scale, f[4 * h + 2] = b.x * scale, f[4 * h + 3] = b.y * scale;
   }
 }
-__device__ __forceinline__ void store_codes(char* base, int64_t i, int n, const float (&y)[8]) {
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {  // (the values are on the e4m3 grid already: the conversion is exact)
-    int t = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
-    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], t, true);
-  }
+__device__ __forceinline__ void store_codes(char* base, int64_t i, int n, const uint32_t (&w)[2]) {
   if (n >= 8) {
     Raw8<uint8_t> r;
     __builtin_memcpy(&r, w, 8);
-    *reinterpret_cast<Raw8<uint8_t>*>(base + i) = r;
+    write8<uint8_t>(base + i, r);
   } else {
     for (int q = 0; q < n; ++q) base[i + q] = (char)(w[q >> 2] >> (8 * (q & 3)));
   }
 }
 
-// maximum over a row of 16 lanes, in every lane of the row
-__device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true)));  // row_ror:8
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true)));  // row_ror:4
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true)));  // row_ror:2
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true)));  // row_ror:1
+// maximum over a row of 16 lanes, in every lane of the row (magnitudes as bit patterns: NaN above infinity above the rest)
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));  // row_ror:8
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));  // row_ror:4
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));  // row_ror:2
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));  // row_ror:1
   return v;
 }
 
 // biased exponent E + 127 of the least E with top 2^-E <= 448 = 1.75 * 2^8, E >= -126; 0 for an empty block
-__device__ __forceinline__ int scale_code(float top) {
-  const uint32_t b = __float_as_uint(top);
-  int s = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return top > 0.f ? max(s, 1) : 0;
+__device__ __forceinline__ int scale_code(uint32_t top) {
+  const int s = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return top ? max(s, 1) : 0;
 }
 
-// y on the e4m3 grid, |y| <= 448: up with the probability of the part that is cut off, from 16 random bits.  Normal values
-// keep 3 bits of mantissa (20 are cut); below 2^-6 the grid is that of the first binade, reached by adding 2^-6.
-template <bool KEEP>
-__device__ __forceinline__ float stochastic(float y, uint32_t bits) {
-  const float a = fabsf(y);
-  const bool low = a < 0x1p-6f;
-  float t = low ? a + 0x1p-6f : a;
-  t = __uint_as_float((__float_as_uint(t) + (bits << 4)) & 0xfff00000u);
-  t = low ? t - 0x1p-6f : t;
-  if (KEEP) t = (t == 0.f && a > 0.f) ? 0x1p-9f : t;
-  t = a < __builtin_inff() ? t : __builtin_nanf("");
-  return __builtin_copysignf(t, y);
-}
-
+// x 2^-E to e4m3 with 16 random bits each (at the top of `bits`): up with the probability of the part that is cut off.  That is
+// the hardware's stochastic conversion, which also turns NaN and infinity into NaN.  KEEP (x >= 0): no value but 0 becomes 0.
 template <bool KEEP>
 __device__ __forceinline__ void quantise8(char* codes, uint8_t* scales, int64_t i, int n, const float (&x)[8],
                                           const uint32_t (&bits)[8]) {
-  float top = 0.f;
+  float m = fabsf(x[0]);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const float a = fabsf(x[q]);
-    top = fmaxf(top, a < __builtin_inff() ? a : 0.f);
+  for (int q = 1; q < 8; ++q) m = __builtin_elementwise_maximum(m, fabsf(x[q]));  // (NaN stays NaN)
+  uint32_t top = row_max(__float_as_uint(m) & 0x7fffffffu);
+  if (__builtin_amdgcn_ballot_w64(top >= 0x7f800000u)) {  // some block has a value that is not finite: leave those out
+    uint32_t t = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t b = __float_as_uint(x[q]) & 0x7fffffffu;
+      t = max(t, b < 0x7f800000u ? b : 0);
+    }
+    top = row_max(t);
   }
-  const int s = scale_code(row_max(top));
+  const int s = scale_code(top);
   const float inv = __uint_as_float((uint32_t)(254 - max(s, 1)) << 23);  // 2^-E (an empty block: any)
-  float y[8];
+  uint32_t w[2] = {0, 0};
+  auto value = [&](int q) {
+    float y = x[q] * inv;
+    // 0 -> 0, what is below the least code -> the least code, the rest (NaN too) as it is
+    if (KEEP) y = __builtin_elementwise_maximum(y, __builtin_elementwise_minimum(y * 0x1p126f, 0x1p-9f));
+    return y;
+  };
 #pragma unroll
-  for (int q = 0; q < 8; ++q) y[q] = stochastic<KEEP>(x[q] * inv, bits[q]);
+  for (int h = 0; h < 2; ++h) {
+    w[h] = __builtin_amdgcn_cvt_sr_fp8_f32(value(4 * h), bits[4 * h], w[h], 0);
+    w[h] = __builtin_amdgcn_cvt_sr_fp8_f32(value(4 * h + 1), bits[4 * h + 1], w[h], 1);
+    w[h] = __builtin_amdgcn_cvt_sr_fp8_f32(value(4 * h + 2), bits[4 * h + 2], w[h], 2);
+    w[h] = __builtin_amdgcn_cvt_sr_fp8_f32(value(4 * h + 3), bits[4 * h + 3], w[h], 3);
+  }
   if (n > 0) {
-    store_codes(codes, i, n, y);
+    store_codes(codes, i, n, w);
     if ((threadIdx.x & 15) == 0) scales[i / BLOCK8] = (uint8_t)s;
   }
 }
 
+// Eight elements per lane from element `start` of the tensor on.  (Lanes behind the end stay: a block's lanes work together.)
 template <typename PT, typename GT, bool EIGHT>
 __device__ __forceinline__ void chunk(const Rec& t, const Args& a, int64_t start) {
-  const int64_t end = min(t.numel, start + a.chunk_elems);
-  for (int64_t i = start + (int64_t)threadIdx.x * VEC; i < start + a.chunk_elems; i += PASS) {
-    if (i - (int64_t)threadIdx.x * VEC >= end) break;  // (uniform: the lanes of a block of 128 stay together)
-    const int n = (int)max((int64_t)0, min((int64_t)VEC, end - i));
-    float p[8], g[8], m[8], v[8], r[8];
-    load8<PT>(t.p, i, n, p);
-    load8<GT>(t.g, i, n, g);
-    if constexpr (EIGHT) {
-      const float sm = n > 0 ? __uint_as_float((uint32_t)t.ms[i / BLOCK8] << 23) : 0.f;
-      const float sv = n > 0 ? __uint_as_float((uint32_t)t.vs[i / BLOCK8] << 23) : 0.f;
-      load_codes(t.m, i, n, sm, m);
-      load_codes(t.v, i, n, sv, r);
+  const int64_t i = start + (int64_t)threadIdx.x * VEC;
+  const int n = (int)max((int64_t)0, min((int64_t)VEC, t.numel - i));
+  float p[8], g[8], m[8], v[8], r[8];
+  load8<PT>(t.p, i, n, p);
+  load8<GT>(t.g, i, n, g);
+  if constexpr (EIGHT) {
+    const float sm = n > 0 ? __uint_as_float((uint32_t)t.ms[i / BLOCK8] << 23) : 0.f;
+    const float sv = n > 0 ? __uint_as_float((uint32_t)t.vs[i / BLOCK8] << 23) : 0.f;
+    load_codes(t.m, i, n, sm, m);
+    load_codes(t.v, i, n, sv, r);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = r[q] * r[q];
-    } else {
-      load8<float>(t.m, i, n, m);
-      load8<float>(t.v, i, n, v);
-    }
+    for (int q = 0; q < 8; ++q) v[q] = r[q] * r[q];
+  } else {
+    load8<float>(t.m, i, n, m);
+    load8<float>(t.v, i, n, v);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    m[q] = fmaf(g[q] - m[q], a.c1, m[q]);
+    v[q] = fmaf(g[q] * a.c2, g[q], v[q] * a.b2);
+    r[q] = __builtin_amdgcn_sqrtf(v[q]);
+    // 1-ulp square root and reciprocal: the update they feed is a small part of p, and r is rounded to 4 bits
+    const float upd = m[q] * __builtin_amdgcn_rcpf(fmaf(r[q], a.inv_sqrt_bc2, a.eps));
+    p[q] = fmaf(-t.step_size, upd, p[q] * t.decay);
+  }
+  store8<PT>(t.p, i, n, p);
+  if constexpr (EIGHT) {
+    uint32_t lo[8], hi[8];
+    const uint32_t seg = (uint32_t)((uint64_t)i >> 32);
+    const uint32_t key = seg == 0 ? t.key : mix32(t.key + seg * 0x9E3779B9u);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      m[q] = fmaf(g[q] - m[q], a.c1, m[q]);
-      v[q] = fmaf(g[q] * a.c2, g[q], v[q] * a.b2);
-      r[q] = __builtin_amdgcn_sqrtf(v[q]);
-      // 1-ulp square root and reciprocal: the update they feed is a small part of p, and r is rounded to 4 bits
-      const float upd = m[q] * __builtin_amdgcn_rcpf(fmaf(r[q], a.inv_sqrt_bc2, a.eps));
-      p[q] = fmaf(-t.step_size, upd, p[q] * t.decay);
+      const uint32_t h = mix32(((uint32_t)i ^ key) ^ q);  // (i is a multiple of 8)
+      lo[q] = h << 16;
+      hi[q] = h & 0xffff0000u;
     }
-    store8<PT>(t.p, i, n, p);
-    if constexpr (EIGHT) {
-      uint32_t lo[8], hi[8];
-      const uint32_t seg = (uint32_t)((uint64_t)i >> 32);
-      const uint32_t key = seg == 0 ? t.key : mix32(t.key + seg * 0x9E3779B9u);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t h = mix32(((uint32_t)i + q) ^ key);
-        lo[q] = h & 0xffffu;
-        hi[q] = h >> 16;
-      }
-      quantise8<false>(t.m, t.ms, i, n, m, lo);
-      quantise8<true>(t.v, t.vs, i, n, r, hi);
-    } else {
-      store8<float>(t.m, i, n, m);
-      store8<float>(t.v, i, n, v);
-    }
+    quantise8<false>(t.m, t.ms, i, n, m, lo);
+    quantise8<true>(t.v, t.vs, i, n, r, hi);
+  } else {
+    store8<float>(t.m, i, n, m);
+    store8<float>(t.v, i, n, v);
   }
 }
 
@@ -228,7 +273,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const Args a) {
     else hi = mid - 1;
   }
   const Rec& t = a.rec[lo];
-  const int64_t start = (int64_t)(blockIdx.x - t.chunk0) * a.chunk_elems;
+  const int64_t start = (int64_t)(blockIdx.x - t.chunk0) * CHUNK;
   const bool eight = t.ms != nullptr;
   if (t.p_dtype == CLT_BF16) {
     if (t.g_dtype == CLT_BF16) {
@@ -273,15 +318,13 @@ extern "C" int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, 
   }
   CLT_CHECK_ARG(total < (1ll << 42), "clt_adamw_step: too many elements");
   const double bc1 = 1.0 - pow(b1, (double)step), bc2 = 1.0 - pow(b2, (double)step);
-  const int chunk_elems = 4 * PASS;
   Args a;
-  a.chunk_elems = chunk_elems;
   a.c1 = (float)(1.0 - b1), a.b2 = (float)b2, a.c2 = (float)(1.0 - b2);
   a.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2)), a.eps = (float)eps;
   a.n = 0;
   uint64_t chunks = 0;
   for (int i = 0; i <= n_tensors; ++i) {
-    const uint64_t mine = i < n_tensors ? ((uint64_t)h_tensors[i].numel + chunk_elems - 1) / chunk_elems : 0;
+    const uint64_t mine = i < n_tensors ? ((uint64_t)h_tensors[i].numel + CHUNK - 1) / CHUNK : 0;
     if (a.n && (i == n_tensors || a.n == MAX_TENSORS || chunks + mine >= (1ull << 31))) {
       hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)chunks), dim3(256), 0, (hipStream_t)stream, a);
       CLT_CHECK_LAUNCH("clt_adamw_step");

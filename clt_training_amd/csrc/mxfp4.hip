@@ -66,50 +66,63 @@ __device__ __forceinline__ void load_row8(const T* row, int64_t c, int64_t K, fl
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t R, int64_t K,
+// Row and column of lane i (8 columns each): FLAT: the rows are contiguous and whole blocks, so no division is needed.
+template <bool FLAT>
+struct Place {
+  int64_t row, c;
+  __device__ __forceinline__ Place(int64_t i, int64_t lanes_per_row, int64_t total) {
+    if (FLAT) {
+      row = 0, c = 8 * i;
+    } else if (total < (1ll << 32)) {
+      const uint32_t r = (uint32_t)i / (uint32_t)lanes_per_row;
+      row = r, c = (int64_t)((uint32_t)i - r * (uint32_t)lanes_per_row) * 8;
+    } else {
+      row = i / lanes_per_row, c = (i - row * lanes_per_row) * 8;
+    }
+  }
+};
+
+template <typename T, bool FLAT>
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t K, int64_t total,
                                                              int64_t lanes_per_row, uint32_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
-  const int64_t total = R * lanes_per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / lanes_per_row, c = (i - row * lanes_per_row) * 8;
-    float f[8];
-    load_row8(x + row * ldx, c, K, f);
-    int s;
-    const uint32_t w = quantise_lane(f, s);  // (a quad of lanes is one block: lanes_per_row is a multiple of 16)
-    codes[i] = w;
-    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
-  }
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;  // (a quad of lanes is one block and goes the same way: total and lanes_per_row are multiples of 16)
+  const Place<FLAT> at(i, lanes_per_row, total);
+  float f[8];
+  load_row8(x + at.row * ldx, at.c, FLAT ? INT64_MAX : K, f);
+  int s;
+  codes[i] = quantise_lane(f, s);
+  if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
 }
 
 // ---- and back --------------------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool FLAT>
 __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes,
-                                                               const uint8_t* __restrict__ scales, int64_t R, int64_t K,
+                                                               const uint8_t* __restrict__ scales, int64_t K, int64_t total,
                                                                int64_t lanes_per_row, T* __restrict__ out) {
-  const int64_t total = R * lanes_per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / lanes_per_row, c = (i - row * lanes_per_row) * 8;
-    if (c >= K) continue;
-    const uint32_t w = codes[i];
-    const int s = scales[i >> 2];
-    float f[8];
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = d.x, f[5] = d.y, f[6] = e.x, f[7] = e.y;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const Place<FLAT> at(i, lanes_per_row, total);
+  if (!FLAT && at.c >= K) return;
+  const uint32_t w = codes[i];
+  const int s = scales[i >> 2];
+  float f[8];
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+  f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = d.x, f[5] = d.y, f[6] = e.x, f[7] = e.y;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) f[q] = s == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(f[q], s - 127);
-    T* o = out + row * K + c;
-    if (c + 8 <= K) {
-      Raw8<T> r;
+  for (int q = 0; q < 8; ++q) f[q] = s == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(f[q], s - 127);
+  T* o = out + at.row * K + at.c;
+  if (FLAT || at.c + 8 <= K) {
+    Raw8<T> r;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) r.e[q] = (T)f[q];
-      *reinterpret_cast<Raw8<T>*>(o) = r;
-    } else {
+    for (int q = 0; q < 8; ++q) r.e[q] = (T)f[q];
+    *reinterpret_cast<Raw8<T>*>(o) = r;
+  } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (c + q < K) o[q] = (T)f[q];
-    }
+    for (int q = 0; q < 8; ++q)
+      if (at.c + q < K) o[q] = (T)f[q];
   }
 }
 
@@ -940,22 +953,29 @@ __global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
 using namespace clt;
 
 static int64_t padded(int64_t K) { return (K + KPAD - 1) / KPAD * KPAD; }
-static unsigned blocks_for(int64_t lanes) { return (unsigned)((lanes + 255) / 256 < 16384 ? (lanes + 255) / 256 : 16384); }
+template <typename T>
+static void launch_quantize(const T* x, int64_t ldx, int64_t R, int64_t K, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  const int64_t lpr = padded(K) / 8, total = R * lpr;
+  const bool flat = K == padded(K) && (ldx == K || R == 1);
+  hipLaunchKernelGGL((flat ? mxfp4_quantize_kernel<T, true> : mxfp4_quantize_kernel<T, false>), dim3((unsigned)((total + 255) / 256)),
+                     dim3(256), 0, st, x, ldx, K, total, lpr, (uint32_t*)codes, scales);
+}
+template <typename T>
+static void launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t K, T* out, hipStream_t st) {
+  const int64_t lpr = padded(K) / 8, total = R * lpr;
+  hipLaunchKernelGGL((K == padded(K) ? mxfp4_dequantize_kernel<T, true> : mxfp4_dequantize_kernel<T, false>),
+                     dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint32_t*)codes, scales, K, total, lpr, out);
+}
 
 extern "C" int clt_mxfp4_quantize(const void* x, int x_dtype, int64_t ldx, int64_t R, int64_t K, uint8_t* codes,
                                   uint8_t* scales, clt_stream_t stream) {
   CLT_CHECK_ARG(x && codes && scales, "clt_mxfp4_quantize: null pointer");
   CLT_CHECK_ARG(valid_dtype(x_dtype), "clt_mxfp4_quantize: dtype");
-  CLT_CHECK_ARG(R > 0 && K > 0 && K < (1ll << 30) && R < (1ll << 40) / K && ldx >= 0, "clt_mxfp4_quantize: bad sizes");
+  CLT_CHECK_ARG(R > 0 && K > 0 && K < (1ll << 30) && R <= (1ll << 39) / padded(K) && ldx >= 0, "clt_mxfp4_quantize: bad sizes");
   CLT_CHECK_ARG(aligned16(codes) && !((uintptr_t)scales & 3) && !((uintptr_t)x & (dtype_size(x_dtype) - 1)),
                 "clt_mxfp4_quantize: misaligned pointer");
-  const int64_t lpr = padded(K) / 8;
-  if (x_dtype == CLT_BF16)
-    hipLaunchKernelGGL(mxfp4_quantize_kernel<bf16_t>, dim3(blocks_for(R * lpr)), dim3(256), 0, (hipStream_t)stream,
-                       (const bf16_t*)x, ldx, R, K, lpr, (uint32_t*)codes, scales);
-  else
-    hipLaunchKernelGGL(mxfp4_quantize_kernel<float>, dim3(blocks_for(R * lpr)), dim3(256), 0, (hipStream_t)stream,
-                       (const float*)x, ldx, R, K, lpr, (uint32_t*)codes, scales);
+  if (x_dtype == CLT_BF16) launch_quantize((const bf16_t*)x, ldx, R, K, codes, scales, (hipStream_t)stream);
+  else launch_quantize((const float*)x, ldx, R, K, codes, scales, (hipStream_t)stream);
   CLT_CHECK_LAUNCH("clt_mxfp4_quantize");
   return CLT_OK;
 }
@@ -964,16 +984,11 @@ extern "C" int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
                                     int out_dtype, clt_stream_t stream) {
   CLT_CHECK_ARG(codes && scales && out, "clt_mxfp4_dequantize: null pointer");
   CLT_CHECK_ARG(valid_dtype(out_dtype), "clt_mxfp4_dequantize: dtype");
-  CLT_CHECK_ARG(R > 0 && K > 0 && K < (1ll << 30) && R < (1ll << 40) / K, "clt_mxfp4_dequantize: bad sizes");
+  CLT_CHECK_ARG(R > 0 && K > 0 && K < (1ll << 30) && R <= (1ll << 39) / padded(K), "clt_mxfp4_dequantize: bad sizes");
   CLT_CHECK_ARG(aligned16(codes) && !((uintptr_t)scales & 3) && !((uintptr_t)out & (dtype_size(out_dtype) - 1)),
                 "clt_mxfp4_dequantize: misaligned pointer");
-  const int64_t lpr = padded(K) / 8;
-  if (out_dtype == CLT_BF16)
-    hipLaunchKernelGGL(mxfp4_dequantize_kernel<bf16_t>, dim3(blocks_for(R * lpr)), dim3(256), 0, (hipStream_t)stream,
-                       (const uint32_t*)codes, scales, R, K, lpr, (bf16_t*)out);
-  else
-    hipLaunchKernelGGL(mxfp4_dequantize_kernel<float>, dim3(blocks_for(R * lpr)), dim3(256), 0, (hipStream_t)stream,
-                       (const uint32_t*)codes, scales, R, K, lpr, (float*)out);
+  if (out_dtype == CLT_BF16) launch_dequantize(codes, scales, R, K, (bf16_t*)out, (hipStream_t)stream);
+  else launch_dequantize(codes, scales, R, K, (float*)out, (hipStream_t)stream);
   CLT_CHECK_LAUNCH("clt_mxfp4_dequantize");
   return CLT_OK;
 }
