@@ -7,21 +7,13 @@
 namespace clt {
 namespace {
 
-#ifndef V_ORDER
-#define V_ORDER 16
-#endif
-#ifndef V_NT
-#define V_NT 0
-#endif
-#ifndef V_SCHED
-#define V_SCHED 1
-#endif
 constexpr int KPAD = 128;  // columns are padded to whole matrix-instruction steps: no bounds in the product's inner loop
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // Eight elements from an address with no more than the element's own alignment.
 template <typename T>
@@ -129,10 +121,16 @@ __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* _
 // ---- product ---------------------------------------------------------------------------------------------------------
 // v_mfma_scale_f32_32x32x64_f8f6f4 with 4-bit operands: lane l of an operand holds row l % 32, columns 32 (l / 32) .. + 31 of
 // a step of 64 -- one block, 16 bytes of codes and one scale.  D: lane l holds column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4.
-__device__ __forceinline__ f32x16 mfma4(const i32x4& a, const i32x4& b, const f32x16& c, int sa, int sb) {
+template <int T>  // 64 columns: byte 2 T of the scales
+__device__ __forceinline__ f32x16 mfma4s(const i32x4& a, const i32x4& b, const f32x16& c, int sa, int sb) {
   const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
   const i32x8 B = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 2 * T, sa, 2 * T, sb);
+}
+
+// (what lies behind `size` reads as zero, dword by dword)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* base, int64_t size) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)max(min(size, (int64_t)0x7fffffff), (int64_t)0), 0x00020000);
 }
 
 struct LinearArgs {
@@ -141,7 +139,24 @@ struct LinearArgs {
   void* out;
   int64_t N, M, ldo;
   int kp, bias_dtype, relu;
+  int lines;  // the rows of out begin with a whole 128-byte line
 };
+
+// 16 bytes of a row to an address with the element's own alignment.  LINES: the row's pieces of 128 bytes are whole lines, and
+// go past L2, where the operands stay (8192 tokens x 98304 x 768, bf16: 552 us, through L2 605; fp32 649, 821).  Else through
+// L2, which joins the parts of a line (2048 x 43579 x 64: 42 us, past it 102).
+typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool LINES>
+__device__ __forceinline__ void store_row16(bf16_t* to, u32x4 w) {
+  if constexpr (LINES) __builtin_nontemporal_store((u32x4_any2)w, reinterpret_cast<u32x4_any2*>(to));
+  else *reinterpret_cast<u32x4_any2*>(to) = (u32x4_any2)w;
+}
+template <bool LINES>
+__device__ __forceinline__ void store_row16(float* to, u32x4 w) {
+  if constexpr (LINES) __builtin_nontemporal_store((u32x4_any4)w, reinterpret_cast<u32x4_any4*>(to));
+  else *reinterpret_cast<u32x4_any4*>(to) = (u32x4_any4)w;
+}
 
 // Few tokens (at most 16 NT): bound by reading W, so W goes from memory to registers once and nothing else is in the way.  A wave
 // takes 16 rows of W at a time (v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, columns 32 (l / 16) .. + 31 of 128),
@@ -155,11 +170,34 @@ __device__ __forceinline__ f32x4 mfma4_16(const i32x4& a, const i32x4& b, const 
   const i32x8 B = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, 0, sa, 0, sb);
 }
-// (what lies behind `size` reads as zero, dword by dword)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* base, int64_t size) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)max(min(size, (int64_t)0x7fffffff), (int64_t)0), 0x00020000);
+// Latents m .. m + 3 of a token: bias, ReLU, one rounding.
+__device__ __forceinline__ f32x4 bias_four(const LinearArgs& p, int64_t m) {
+  f32x4 b = {};
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = load_scalar(p.bias, p.bias_dtype, min(m + i, p.M - 1));
+  }
+  return b;
 }
-
+template <typename T>
+__device__ __forceinline__ void store_four(const LinearArgs& p, T* row, int64_t m, const f32x4& acc, const f32x4& b) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T e[4];
+  };
+  Four o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = acc[i] + b[i];
+    o.e[i] = (T)(p.relu ? __builtin_elementwise_maximum(v, 0.f) : v);
+  }
+  if (m + 4 <= p.M) {
+    *reinterpret_cast<Four*>(row + m) = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (m + i < p.M) row[m + i] = o.e[i];
+  }
+}
 template <typename XT, typename T, int NT>
 __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, const XT* __restrict__ x, int64_t ldx, int K) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -206,9 +244,7 @@ __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, cons
   load(g, 0, now);
   while (g < groups) {
     const int64_t m = g * 16 + 4 * q;  // this lane's four latents
-    float b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = p.bias ? load_scalar(p.bias, p.bias_dtype, min(m + i, p.M - 1)) : 0.f;
+    const f32x4 b = bias_four(p, m);
     f32x4 acc[NT] = {};
     const int64_t next = g + step;
     for (int c = 0; c < nch; ++c) {
@@ -230,93 +266,29 @@ __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, cons
     for (int t = 0; t < NT; ++t) {
       const int n = 16 * t + r16;
       if (n >= N) continue;
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = acc[t][i] + b[i];
-        if (p.relu) v[i] = __builtin_elementwise_maximum(v[i], 0.f);
-      }
-      T* to = out + n * p.ldo + m;
-      if (m + 4 <= p.M) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Four {
-          T e[4];
-        };
-        Four o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o.e[i] = (T)v[i];
-        *reinterpret_cast<Four*>(to) = o;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (m + i < p.M) to[i] = (T)v[i];
-      }
+      store_four(p, out + n * p.ldo, m, acc[t], b);
     }
     g = next;
   }
 }
 
-// One wave per 32 latents x 32 tokens, operands straight from memory.
-template <typename T>
-__global__ __launch_bounds__(64) void mxfp4_linear_kernel(const LinearArgs p) {
-  const int lane = threadIdx.x, r = lane & 31, h = lane >> 5;
-  const int64_t m0 = (int64_t)blockIdx.x * 32, n0 = (int64_t)blockIdx.y * 32;
-  const int64_t wr = min(m0 + r, p.M - 1), xr = min(n0 + r, p.N - 1);
-  const uint8_t* wc = p.wc + wr * (p.kp / 2) + 16 * h;
-  const uint8_t* xc = p.xc + xr * (p.kp / 2) + 16 * h;
-  const uint8_t* ws = p.ws + wr * (p.kp / 32) + h;
-  const uint8_t* xs = p.xs + xr * (p.kp / 32) + h;
-  f32x16 acc = {};
-  for (int k = 0; k < p.kp / 64; ++k)
-    acc = mfma4(*(const i32x4*)(xc + 32 * k), *(const i32x4*)(wc + 32 * k), acc, xs[2 * k], ws[2 * k]);
-  const int64_t m = m0 + r;
-  if (m >= p.M) return;
-  const float b = p.bias ? load_scalar(p.bias, p.bias_dtype, m) : 0.f;
-  T* out = reinterpret_cast<T*>(p.out);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t n = n0 + 8 * (i / 4) + 4 * h + i % 4;
-    float v = acc[i] + b;
-    if (p.relu) v = v < 0.f ? 0.f : v;
-    if (n < p.N) out[n * p.ldo + m] = (T)v;
-  }
-}
-
-
-// Large problems.  A workgroup of four waves computes 256 latents x 128 tokens, a wave 128 x 64 of them (4 x 2 tiles of
-// 32 x 32, 128 accumulators), so that two workgroups share a CU: the waits, the first loads and the stores of one run
-// beside the matrix instructions of the other.
-//
-// Per stage of 128 columns both operands come as rows of 64 bytes by LDS-DMA (24 pieces of 16 rows = 1 KiB, six per wave)
-// into a ring of three slots, two stages ahead; one barrier per stage.  A lane of a piece fetches the 16-byte chunk c =
-// (lane % 4) ^ (row / 4 % 4) of its row: the fragment reads (lane l: row l % 32, chunk 2 t + l / 32) then touch every bank once.
-// The scales of four stages are 16 bytes of a row: one DMA for 64 rows, then four registers per fragment row.
-// The finished tile goes through the ring's LDS once, so that a store instruction writes rows of 256 bytes.
-constexpr int TM = 256, TN = 128, KS = 128;
-constexpr int STAGE_W = TM * 64, STAGE_BYTES = (TM + TN) * 64, NSLOT = 3;
-constexpr int SCALE_OFF = NSLOT * STAGE_BYTES, TILE_LDS = SCALE_OFF + (TM + TN) * 16;
-constexpr int PITCH = 272;                       // bytes between the token rows of the transposed tile (256 of data)
-constexpr int BIAS_OFF = 4 * 32 * PITCH;
-constexpr int PANEL = 16;                        // token tiles that share their operand rows in an XCD's L2
-static_assert(BIAS_OFF + TM * 4 <= TILE_LDS && 2 * TILE_LDS <= 160 * 1024, "LDS");
+// Middle-sized problems.  A workgroup of four waves computes 128 latents x 128 tokens, a wave 64 x 64 of them; two workgroups
+// share a CU, so that the waits, the first loads and the stores of one run beside the matrix instructions of the other.  Per
+// stage of 256 columns both operands come as whole lines of 128 bytes by LDS-DMA into a ring of two slots, one stage ahead; what
+// lies behind an array's last row reads as zeros.  Chunk c of a row lies at c ^ (row / 2 % 8): fragment reads (16 rows, one
+// chunk) hit every bank once.  The finished tile goes through the ring's LDS once, so that a store instruction writes rows of
+// 128 bytes and more.
+//   Bound by the time a stage takes from its fetch to its use (about 0.7 us a stage with one workgroup a CU) while tiles are
+// fewer than 512, then by LDS and the matrix instructions together.  512 tokens x 6151 x 4096: 18 us; 256 x 128 tiles with
+// stages of 128 columns took 28, three or four slots with one workgroup a CU 17 and up to 1.7 x these times where tiles are many;
+// a second barrier that lets a slot be refilled a step earlier saves 15 % where W comes from HBM for one row of tiles
+// (128 x 98304 x 768: 18 for 21 us) and costs 3 to 9 % elsewhere.
+constexpr int TM = 128, TN = 128, KS = 256, SLOT = (TM + TN) * (128 + 16);
+constexpr int BPANEL = 16;                       // latent tiles that run through all tokens together
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// LDS[lds_dst + 16 * lane] = *(sbase + voff)
-__device__ __forceinline__ void dma16(const uint8_t* sbase, uint32_t voff, uint32_t lds_dst) {
-  unsigned keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(keep)
-      : "v"(voff), "s"(sbase), "s"(lds_dst)
-      : "memory");
-}
-
-// The same from a buffer of `size` bytes: what lies behind its end reads as zero.
 __device__ __forceinline__ i32x4 buffer_of(const uint8_t* base, int64_t size) {
   const uint64_t a = (uint64_t)base;
   i32x4 r;
@@ -326,6 +298,7 @@ __device__ __forceinline__ i32x4 buffer_of(const uint8_t* base, int64_t size) {
   r[3] = 0x00020000;
   return r;
 }
+// LDS[lds_dst + 16 * lane] = buf[voff .. voff + 15]; what lies behind the buffer's end reads as zero.
 __device__ __forceinline__ void dma16_buffer(const i32x4& buf, uint32_t voff, uint32_t lds_dst) {
   unsigned keep;
   asm volatile(
@@ -336,6 +309,22 @@ __device__ __forceinline__ void dma16_buffer(const i32x4& buf, uint32_t voff, ui
       "s_mov_b32 m0, %0"
       : "=&s"(keep)
       : "v"(voff), "s"(buf), "s"(lds_dst)
+      : "memory");
+}
+
+// The same for some of the lanes (all lanes are active where this stands).
+__device__ __forceinline__ void dma16_lanes(const i32x4& buf, uint32_t voff, uint32_t lds_dst, int low, int high) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_mov_b32 exec_lo, %4\n\t"
+      "s_mov_b32 exec_hi, %5\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+      "s_mov_b64 exec, -1\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(buf), "s"(lds_dst), "i"(low), "i"(high)
       : "memory");
 }
 
@@ -367,24 +356,6 @@ __device__ __forceinline__ void dma4_masked(const i32x4& buf, uint32_t voff, uin
       : "=&s"(keep)
       : "v"(voff), "s"(buf), "s"(lds_dst), "s"(mask)
       : "memory");
-}
-
-template <int T>  // half of a stage: 64 columns
-__device__ __forceinline__ f32x16 mfma4s(const i32x4& a, const i32x4& b, const f32x16& c, int sa, int sb) {
-  const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
-  const i32x8 B = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, c, 4, 4, 2 * T, sa, 2 * T, sb);
-}
-
-// 16 bytes to an address with the element's own alignment, past L2's lines: for stores that write whole 128-byte lines
-// (5.2 TB/s either way, and the operands stay in L2; rows of 64 bytes would reach 2.9 TB/s).
-typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
-__device__ __forceinline__ void store_row16(bf16_t* to, u32x4 w) {
-  __builtin_nontemporal_store((u32x4_any2)w, reinterpret_cast<u32x4_any2*>(to));
-}
-__device__ __forceinline__ void store_row16(float* to, u32x4 w) {
-  __builtin_nontemporal_store((u32x4_any4)w, reinterpret_cast<u32x4_any4*>(to));
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -438,230 +409,229 @@ __device__ __forceinline__ void lines_of(u32x4 (&c)[8]) {
 
 template <typename T>
 __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) {
-  __shared__ __attribute__((aligned(1024))) char lds[TILE_LDS];
+  static_assert(2 * 2 * SLOT <= 160 * 1024, "LDS of two workgroups");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
 
-  // ---- tile: an XCD (workgroup id % 8) owns a contiguous range of positions; a panel of token tiles runs through all latents
+  // ---- tile: an XCD (workgroup id % 8) owns a contiguous range of positions; a panel of latent tiles runs through all tokens
   const int64_t nlt = (p.M + TM - 1) / TM, ntt = (p.N + TN - 1) / TN, ntiles = nlt * ntt;
   const int64_t xg = blockIdx.x & 7, q = ntiles >> 3, rest = ntiles & 7;
   const int64_t pos = xg * q + min(xg, rest) + (blockIdx.x >> 3);
-#if V_ORDER == 0
-  const int64_t panel = pos / (nlt * PANEL), in = pos - panel * nlt * PANEL;
-  const int64_t width = min((int64_t)PANEL, ntt - panel * PANEL);
-  const int64_t m0 = in / width * TM, n0 = (panel * PANEL + in % width) * TN;
-#else
-  const int64_t panel = pos / (ntt * V_ORDER), in = pos - panel * ntt * V_ORDER;
-  const int64_t width = min((int64_t)V_ORDER, nlt - panel * V_ORDER);
-  const int64_t n0 = in / width * TN, m0 = (panel * V_ORDER + in % width) * TM;
-#endif
+  const int64_t panel = pos / (ntt * BPANEL), in = pos - panel * ntt * BPANEL;
+  const int64_t width = min((int64_t)BPANEL, nlt - panel * BPANEL);
+  const int64_t n0 = in / width * TN, m0 = (panel * BPANEL + in % width) * TM;
 
-  // ---- loader: this wave's pieces of a stage (four of W, two of x), rows past the end read the last one again
-  const int rowb = p.kp / 2, sb = p.kp / 32, nst = p.kp / KS;
-  const uint8_t* wbase = p.wc + m0 * rowb;
-  const uint8_t* xbase = p.xc + n0 * rowb;
-  const int wleft = (int)min((int64_t)TM, p.M - m0) - 1, xleft = (int)min((int64_t)TN, p.N - n0) - 1;
-  uint32_t woff[4], xoff[2];
+  // ---- loader: 64 rows a wave (waves 0, 1: W, 2, 3: x), eight pieces of eight rows and their scales
+  const int rowb = p.kp / 2, sb = p.kp / 32, nst = (p.kp + KS - 1) / KS;
+  const int64_t row0 = (wave < 2 ? m0 : n0) + 64 * (wave & 1), left = max((wave < 2 ? p.M : p.N) - row0, (int64_t)0);
+  const i32x4 cbuf = buffer_of((wave < 2 ? p.wc : p.xc) + row0 * rowb, left * rowb);
+  const i32x4 sbuf = buffer_of((wave < 2 ? p.ws : p.xs) + row0 * sb, left * sb);
+  const uint32_t chunk = ((lane & 7) ^ (lane >> 4)) << 4;
+  const uint32_t even = (uint32_t)(lane >> 3) * rowb + chunk, odd = even - chunk + (chunk ^ 64);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + wave * 8192;
+  const uint32_t sc0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + (TM + TN) * 128 + wave * 1024;
+  auto fetch = [&](int s, int slot) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (4 * wave + i) * 16 + (lane >> 2);
-    woff[i] = (uint32_t)min(row, wleft) * rowb + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = (2 * wave + i) * 16 + (lane >> 2);
-    xoff[i] = (uint32_t)min(row, xleft) * rowb + (((lane & 3) ^ ((row >> 2) & 3)) << 4);
-  }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  auto load_stage = [&](int s, int slot) {
-    const uint32_t d = lds0 + slot * STAGE_BYTES;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dma16(wbase + (int64_t)s * 64, woff[i], d + (4 * wave + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) dma16(xbase + (int64_t)s * 64, xoff[i], d + STAGE_W + (2 * wave + i) * 1024);
+    for (int i = 0; i < 8; ++i)
+      dma16_buffer(cbuf, ((i & 1) ? odd : even) + (uint32_t)(128 * s + i * 8 * rowb), lds0 + slot * SLOT + i * 1024);
+    dma16_buffer(sbuf, (uint32_t)(lane * sb + 8 * s), sc0 + slot * SLOT);
   };
-  // The scales of a row end behind 16 bytes of the last chunk: what follows is the next row's.  Only behind the last row
-  // there is nothing; there the 16 bytes are taken from further left (`back`) and moved into place when they are read.
-  const uint8_t* wsc = p.ws + m0 * sb;
-  const uint8_t* xsc = p.xs + n0 * sb;
-  const int64_t wend = (p.M - m0) * sb - 16, xend = (p.N - n0) * sb - 16;  // (last position that 16 bytes may be read from)
-  auto load_scales = [&](int c) {
+
+  // ---- multiplier
+  f32x16 acc[2][2] = {};  // [latents][tokens]; lane (r32, h): token r32, latents 8 g + 4 h + j
+  const uint32_t at = r32 * 128 + ((h ^ (r32 >> 1 & 7)) << 4);
+  const uint32_t wat = wm * 8192 + at, xat = (2 + wn) * 8192 + at;
+  fetch(0, 0);
+  for (int s = 0; s < nst; ++s) {
+    // stage s is there, and every wave is past stage s - 1
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + 1 < nst) fetch(s + 1, ~s & 1);
+    const char* base = lds + (s & 1) * SLOT;
+    i32x4 w[2][4], x[2][4];
+    u32x2 sw[2], sx[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int piece = wave + 4 * i;  // 0 .. 3: W, 4 .. 5: x
-      if (piece >= 6) break;
-      const bool w = piece < 4;
-      const int row = min((w ? piece : piece - 4) * 64 + lane, w ? wleft : xleft);
-      const int64_t off = min((int64_t)row * sb + 16 * c, w ? wend : xend);
-      // (off may be negative: the base lies inside the array, 16 bytes before its end are inside it too)
-      const uint8_t* base = w ? wsc : xsc;
-      const uint8_t* low = base + min((int64_t)0, w ? wend : xend);
-      dma16(low, (uint32_t)(base + off - low), lds0 + SCALE_OFF + piece * 1024);
+      sw[i] = *reinterpret_cast<const u32x2*>(base + (TM + TN) * 128 + (wm * 64 + 32 * i + r32) * 16);
+      sx[i] = *reinterpret_cast<const u32x2*>(base + (TM + TN) * 128 + (TM + wn * 64 + 32 * i + r32) * 16);
     }
-  };
-  const bool last = m0 + TM >= p.M || n0 + TN >= p.N;  // this tile holds a last row: some scales may lie `back` registers off
-  auto read_scales = [&](int lds_row) { return *reinterpret_cast<const i32x4*>(lds + SCALE_OFF + lds_row * 16); };
-  auto settle = [&](i32x4 v, int row, int c, int left, int64_t end) {
-    const int64_t over = (int64_t)min(row, left) * sb + 16 * c - end;
-    const int back = over > 0 ? (int)over >> 2 : 0;
-    i32x4 u;
-    u[0] = back == 0 ? v[0] : back == 1 ? v[1] : back == 2 ? v[2] : v[3];
-    u[1] = back == 0 ? v[1] : back == 1 ? v[2] : v[3];
-    u[2] = back == 0 ? v[2] : v[3];
-    u[3] = v[3];
-    return u;
-  };
-
-  f32x16 acc[4][2] = {};
-  i32x4 sw[4], sx[2];
-  uint32_t fa[2], fb[2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const uint32_t o = r32 * 64 + (((2 * t + h) ^ ((r32 >> 2) & 3)) << 4);
-    fa[t] = o + wm * 128 * 64;
-    fb[t] = o + STAGE_W + wn * 64 * 64;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[i][j] = *reinterpret_cast<const i32x4*>(base + i * 4096 + (wat ^ (32 * j)));
+        x[i][j] = *reinterpret_cast<const i32x4*>(base + i * 4096 + (xat ^ (32 * j)));
+      }
+    const bool cut = 256 * s + 128 >= p.kp;  // (behind a row's last 128 columns stands the next row: counted 2^-254 times)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sw[i][1] = cut ? 0 : sw[i][1];
+      sx[i][1] = cut ? 0 : sx[i][1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int s1 = (int)(sw[i][j >> 1] >> (8 * h)), s2 = (int)(sx[k][j >> 1] >> (8 * h));
+          acc[i][k] = j & 1 ? mfma4s<1>(w[i][j], x[k][j], acc[i][k], s1, s2) : mfma4s<0>(w[i][j], x[k][j], acc[i][k], s1, s2);
+        }
   }
 
-  load_scales(0);
-  load_stage(0, 0);
-  if (nst > 1) load_stage(1, 1);
-  int slot = 0;
-  for (int s0 = 0; s0 < nst; s0 += 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int s = s0 + j;
-      if (s >= nst) break;
-      // stage s is there when at most the six pieces of stage s + 1 are on their way
-      if (s + 1 < nst) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 2 < nst) {
-        if (j == 2) load_scales((s + 2) >> 2);
-        load_stage(s + 2, slot == 0 ? 2 : slot - 1);  // the slot of stage s - 1: every wave is past it
-      }
-      if (j == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sw[i] = read_scales(wm * 128 + i * 32 + r32);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) sx[i] = read_scales(TM + wn * 64 + i * 32 + r32);
-        if (last) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sw[i] = settle(sw[i], wm * 128 + i * 32 + r32, s0 >> 2, wleft, wend);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) sx[i] = settle(sx[i], wn * 64 + i * 32 + r32, s0 >> 2, xleft, xend);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // bytes 0 and 2: this lane's blocks of the two halves of a stage
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sw[i][e] = (int)((uint32_t)sw[i][e] >> (8 * h));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) sx[i][e] = (int)((uint32_t)sx[i][e] >> (8 * h));
-        }
-      }
-      const char* st = lds + slot * STAGE_BYTES;
-      i32x4 A[2][4], B[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) A[t][i] = *reinterpret_cast<const i32x4*>(st + fa[t] + i * 2048);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) B[t][i] = *reinterpret_cast<const i32x4*>(st + fb[t] + i * 2048);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) acc[i][k] = mfma4s<0>(A[0][i], B[0][k], acc[i][k], sw[i][j], sx[k][j]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) acc[i][k] = mfma4s<1>(A[1][i], B[1][k], acc[i][k], sw[i][j], sx[k][j]);
-#if V_SCHED == 1  // six reads, then one read of the second half behind each of the first matrix instructions
-      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-      for (int e = 0; e < 6; ++e) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 10, 0);
-#elif V_SCHED == 2
-      __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);
-#endif
-      slot = slot == 2 ? 0 : slot + 1;
-    }
-  }
-
-  // ---- epilogue: bias, ReLU, one rounding; lane l of D holds token l % 32, latents 8 (i / 4) + 4 h + i % 4
+  // ---- epilogue: bias, ReLU, one rounding
   __syncthreads();  // (the ring is free)
-  float* bias = reinterpret_cast<float*>(lds + BIAS_OFF);
-  {
+  constexpr int OPITCH = 64 * sizeof(T) + 16, VEC = 16 / sizeof(T), ROWL = 64 / VEC, ROWS = 64 / ROWL;
+  float* bias = reinterpret_cast<float*>(lds + 4 * 32 * OPITCH);
+  if (threadIdx.x < TM) {
     const int64_t m = m0 + threadIdx.x;
     bias[threadIdx.x] = p.bias && m < p.M ? load_scalar(p.bias, p.bias_dtype, m) : 0.f;
   }
   __syncthreads();
-  char* mine = lds + wave * 32 * PITCH;
-  constexpr int LAT = 256 / sizeof(T);            // latents in a row of the transposed tile
-  constexpr int RT = LAT / 32, VEC = 16 / sizeof(T);
+  char* mine = lds + wave * 32 * OPITCH;
   T* out = reinterpret_cast<T*>(p.out);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
 #pragma unroll
-    for (int part = 0; part < 4 / RT; ++part) {
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
+      for (int g = 0; g < 4; ++g) {
+        const int lat = i * 32 + 8 * g + 4 * h;
+        const float4 b = *reinterpret_cast<const float4*>(bias + wm * 64 + lat);
+        float v[4] = {acc[i][k][4 * g] + b.x, acc[i][k][4 * g + 1] + b.y, acc[i][k][4 * g + 2] + b.z, acc[i][k][4 * g + 3] + b.w};
+        if (p.relu) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int lat = (part * RT + i) * 32 + 8 * g + 4 * h;
-          const float4 b = *reinterpret_cast<const float4*>(bias + wm * 128 + lat);
-          float v[4] = {acc[part * RT + i][k][4 * g] + b.x, acc[part * RT + i][k][4 * g + 1] + b.y,
-                        acc[part * RT + i][k][4 * g + 2] + b.z, acc[part * RT + i][k][4 * g + 3] + b.w};
-          if (p.relu) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
-          }
-          char* to = mine + r32 * PITCH + (i * 32 + 8 * g + 4 * h) * sizeof(T);
-          if constexpr (sizeof(T) == 2) {
-            uint2 w;
-            w.x = pack_bf16x2(v[0], v[1]), w.y = pack_bf16x2(v[2], v[3]);
-            *reinterpret_cast<uint2*>(to) = w;
-          } else {
-            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-          }
+          for (int e = 0; e < 4; ++e) v[e] = __builtin_elementwise_maximum(v[e], 0.f);
         }
-      }
-      asm volatile("" ::: "memory");  // (one wave, and a wave's LDS accesses are carried out in order)
-      __builtin_amdgcn_wave_barrier();
-      const int64_t m = m0 + wm * 128 + part * LAT + (lane & 15) * VEC;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int tok = 4 * i + (lane >> 4);
-        const uint4 w = *reinterpret_cast<const uint4*>(mine + tok * PITCH + (lane & 15) * 16);
-        const int64_t n = n0 + wn * 64 + k * 32 + tok;
-        if (n >= p.N) continue;
-        T* to = out + n * p.ldo + m;
-        struct __attribute__((packed, aligned(sizeof(T)))) Row {
-          uint4 w;
-        };
-        if (m + VEC <= p.M) {
-#if V_NT
-          typedef uint32_t nt4 __attribute__((ext_vector_type(4), aligned(4)));
-          __builtin_nontemporal_store(__builtin_bit_cast(u32x4, w), reinterpret_cast<u32x4*>(to));
-#else
-          reinterpret_cast<Row*>(to)->w = w;
-#endif
+        char* to = mine + r32 * OPITCH + lat * sizeof(T);
+        if constexpr (sizeof(T) == 2) {
+          uint2 w;
+          w.x = pack_bf16x2(v[0], v[1]), w.y = pack_bf16x2(v[2], v[3]);
+          *reinterpret_cast<uint2*>(to) = w;
         } else {
-          T e[VEC];
-          __builtin_memcpy(e, &w, 16);
-#pragma unroll
-          for (int c = 0; c < VEC; ++c)
-            if (m + c < p.M) to[c] = e[c];
+          *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
         }
       }
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_wave_barrier();
     }
+    asm volatile("" ::: "memory");  // (one wave, and a wave's LDS accesses are carried out in order)
+    __builtin_amdgcn_wave_barrier();
+    const int64_t m = m0 + wm * 64 + (lane % ROWL) * VEC;
+#pragma unroll
+    for (int i = 0; i < 32 / ROWS; ++i) {
+      const int tok = ROWS * i + lane / ROWL;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(mine + tok * OPITCH + (lane % ROWL) * 16);
+      const int64_t n = n0 + wn * 64 + k * 32 + tok;
+      if (n >= p.N) continue;
+      T* to = out + n * p.ldo + m;
+      if (m + VEC <= p.M) {
+        store_row16<false>(to, w);
+      } else {
+        T e[VEC];
+        __builtin_memcpy(e, &w, 16);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c)
+          if (m + c < p.M) to[c] = e[c];
+      }
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
+// Problems of few tiles.  32 latents x 32 tokens by S of the four waves, each with a contiguous part of the columns; they add
+// up in LDS, in their order.  A wave works by itself: it fetches its rows 256 columns at a time, whole lines of 128 bytes, into
+// two slots of its own, so that no barrier stands in the loop.  (With fragments straight from memory, 16 lanes that are served
+// together read 16 lines: four times the accesses, and 11.8 us instead of 7.2 for 509 tokens x 884 x 4096.)
+// Bound by the loads' latency, from about four workgroups a CU on by their number of bytes (43 bytes a clock and CU).
+constexpr int SB_ROW = 16;  // bytes of scales kept with a row and 256 columns (8 are its own)
+template <typename T, int S>
+__global__ __launch_bounds__(256) void mxfp4_split_kernel(const LinearArgs p) {
+  constexpr int ROWS = 32, CODES = 2 * ROWS * 128, SLOT = CODES + 2 * ROWS * SB_ROW, PIECES = 2 * ROWS / 8 + 2;
+  constexpr int PITCH = ROWS + 8;  // of the sums, in floats
+  static_assert(ROWS * PITCH * 4 <= 2 * SLOT && 8 * SLOT <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) char lds[8 * SLOT];
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int turn = wave % S;
+  char* own = lds + wave * 2 * SLOT;
+  const uint32_t own0 = (uint32_t)(uintptr_t)(lds_ptr_t)own;
+
+  // ---- tile: an XCD (workgroup id % 8) owns a contiguous range, tokens fastest: W comes to one L2 only
+  const int64_t nlt = (p.M + ROWS * (4 / S) - 1) / (ROWS * (4 / S)), ntt = (p.N + ROWS - 1) / ROWS, ntiles = nlt * ntt;
+  const int64_t xg = blockIdx.x & 7, share = ntiles >> 3, rest = ntiles & 7;
+  const int64_t pos = xg * share + min(xg, rest) + (blockIdx.x >> 3);
+  const int64_t m0 = (pos / ntt * (4 / S) + wave / S) * ROWS, n0 = pos % ntt * ROWS;
+
+  const int rowb = p.kp / 2, sb = p.kp / 32, nch = (p.kp + 255) / 256, per = (nch + S - 1) / S;
+  const int first = turn * per, stop = min(nch, first + per);
+  const int64_t mleft = max(p.M - m0, (int64_t)0), nleft = p.N - n0;
+  const i32x4 wbuf = buffer_of(p.wc + m0 * rowb, mleft * rowb), xbuf = buffer_of(p.xc + n0 * rowb, nleft * rowb);
+  const i32x4 wsbuf = buffer_of(p.ws + m0 * sb, mleft * sb), xsbuf = buffer_of(p.xs + n0 * sb, nleft * sb);
+  auto none = [](i32x4 buf, bool on) {
+    buf[2] = on ? buf[2] : 0;
+    return buf;
+  };
+  // Chunk c of a row lies at c ^ (row / 2 % 8): fragment reads (16 rows, one chunk) hit every bank once.
+  const uint32_t chunk = ((lane & 7) ^ (lane >> 4)) << 4;
+  const uint32_t even = (uint32_t)(lane >> 3) * rowb + chunk, odd = even - chunk + (chunk ^ 64);
+  auto fetch = [&](int c, int slot) {  // (behind `stop`: zeros, so that the pieces in flight are always as many)
+    const bool on = c < stop;
+    const i32x4 wb = none(wbuf, on), xb = none(xbuf, on);
+    const uint32_t to = own0 + slot * SLOT;
+#pragma unroll
+    for (int i = 0; i < 2 * ROWS / 8; ++i) {  // eight rows each: W's, then x's
+      const int piece = i % (ROWS / 8);
+      dma16_buffer(i < ROWS / 8 ? wb : xb, ((piece & 1) ? odd : even) + (uint32_t)(128 * c + piece * 8 * rowb), to + i * 1024);
+    }
+    dma16_lanes(none(wsbuf, on), (uint32_t)(r * sb + 8 * c), to + CODES, -1, 0);
+    dma16_lanes(none(xsbuf, on), (uint32_t)(r * sb + 8 * c), to + CODES, 0, -1);
+  };
+  f32x16 acc = {};  // lane (r, h): latent r, tokens 8 g + 4 h + j
+  const uint32_t at = r * 128 + ((h ^ (r >> 1 & 7)) << 4);
+  auto multiply = [&](int c, int slot) {
+    const char* base = own + slot * SLOT;
+    i32x4 w[4], x[4];
+    u32x2 sw = *reinterpret_cast<const u32x2*>(base + CODES + r * SB_ROW);
+    u32x2 sx = *reinterpret_cast<const u32x2*>(base + CODES + (ROWS + r) * SB_ROW);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = *reinterpret_cast<const i32x4*>(base + (at ^ (32 * j)));
+      x[j] = *reinterpret_cast<const i32x4*>(base + ROWS * 128 + (at ^ (32 * j)));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is free
+    fetch(c + 2, slot);
+    if (256 * c + 128 >= p.kp) sw[1] = sx[1] = 0;  // (behind a row's last 128 columns stands the next row: counted 2^-254 times)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int s1 = (int)(sx[j >> 1] >> (8 * h)), s2 = (int)(sw[j >> 1] >> (8 * h));
+      acc = j & 1 ? mfma4s<1>(x[j], w[j], acc, s1, s2) : mfma4s<0>(x[j], w[j], acc, s1, s2);
+    }
+  };
+  if (first < stop && mleft) {
+    fetch(first, 0);
+    fetch(first + 1, 1);
+    for (int c = first; c < stop; ++c) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+      multiply(c, (c - first) & 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the sums go where the slots are)
+  }
+  float* sums = reinterpret_cast<float*>(own);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sums[(8 * (e / 4) + 4 * h + e % 4) * PITCH + r] = acc[e];
+  __syncthreads();
+  // four latents of a token per thread
+  T* out = reinterpret_cast<T*>(p.out);
+  const char* parts = lds + (wave - turn) * 2 * SLOT;
+  constexpr int QUADS = ROWS / 4;
+#pragma unroll
+  for (int e = 0; e < ROWS * QUADS / (64 * S); ++e) {
+    const int item = e * 64 * S + turn * 64 + lane, n = item / QUADS, m = item % QUADS * 4;
+    f32x4 v = *reinterpret_cast<const f32x4*>(parts + (n * PITCH + m) * 4);
+#pragma unroll
+    for (int k = 1; k < S; ++k) v += *reinterpret_cast<const f32x4*>(parts + k * 2 * SLOT + (n * PITCH + m) * 4);
+    if (n < nleft && m < mleft) store_four(p, out + (n0 + n) * p.ldo, m0 + m, v, bias_four(p, m0 + m));
+  }
+}
 
 // The largest problems.  One persistent workgroup of eight waves per CU computes tiles of 256 latents x 256 tokens (a wave
 // 128 x 64: 4 x 2 tiles of 32 x 32, 128 accumulators, two waves per SIMD).
@@ -710,12 +680,12 @@ __global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
   int pos = xstart + (blockIdx.x >> 3);
   if (pos >= xstop) return;
   auto place = [&](int at, int64_t& m0, int64_t& n0) {
-    const uint32_t full = (uint32_t)ntt * V_ORDER;
+    const uint32_t full = (uint32_t)ntt * BPANEL;
     const uint32_t panel = (uint32_t)at / full, in = (uint32_t)at - panel * full;
-    const uint32_t width = min((uint32_t)V_ORDER, (uint32_t)nlt - panel * V_ORDER);
+    const uint32_t width = min((uint32_t)BPANEL, (uint32_t)nlt - panel * BPANEL);
     const uint32_t row = in / width;
     n0 = (int64_t)__builtin_amdgcn_readfirstlane(row) * BN;
-    m0 = (int64_t)__builtin_amdgcn_readfirstlane(panel * V_ORDER + in - row * width) * BM;
+    m0 = (int64_t)__builtin_amdgcn_readfirstlane(panel * BPANEL + in - row * width) * BM;
   };
 
   // ---- loader: runs two stages ahead of the multiplier.  What lies behind an array's end reads as zero (dword by dword).
@@ -887,7 +857,7 @@ __global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
     const bool whole = m0 + BM <= p.M && n0 + BN <= p.N;
     char* tile_out = reinterpret_cast<char*>(out + n0 * p.ldo + m0);  // (host: 256 rows are less than 2 GiB)
     const int nleft = (int)min(p.N - n0, (int64_t)BN), mleft = (int)min(p.M - m0, (int64_t)BM);
-    auto finish = [&](auto whole_) {
+    auto finish = [&](auto whole_, auto lines_) {
 #pragma unroll
       for (int part = 0; part < (int)sizeof(T) / 2; ++part) {  // 128 bytes of every token: 64 or 32 latents of each half
 #pragma unroll
@@ -919,10 +889,10 @@ __global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
             const int n = 32 * k + 16 * (s >> 2) + (s & 3), m = part * 32;  // how far this line is from the lane's first one
             T* to = reinterpret_cast<T*>(tile_out + (uint32_t)(n * (int)p.ldo + m) * (uint32_t)sizeof(T) + lane_out);
             if (decltype(whole_)::value) {
-              store_row16(to, c[s]);
+              store_row16<decltype(lines_)::value>(to, c[s]);
             } else if (nl + n < nleft) {
               if (ml + m + VEC <= mleft) {
-                store_row16(to, c[s]);
+                store_row16<false>(to, c[s]);
               } else {
                 T e[VEC];
                 const u32x4 w = c[s];
@@ -936,8 +906,9 @@ __global__ __launch_bounds__(512) void mxfp4_big_kernel(const LinearArgs p) {
         }
       }
     };
-    if (whole) finish(std::true_type{});
-    else finish(std::false_type{});
+    if (whole && p.lines) finish(std::true_type{}, std::true_type{});
+    else if (whole) finish(std::true_type{}, std::false_type{});
+    else finish(std::false_type{}, std::false_type{});
     pos += nbx;
     if (pos >= xstop) break;
     place(pos, m0, n0);
@@ -1002,8 +973,13 @@ int few_tiles(int64_t N, int kp) {
   const int nt = N <= 16 ? 1 : N <= 32 ? 2 : N <= 64 ? 4 : 0;
   return nt && few_lds(nt, kp) <= FEW_LDS ? nt : 0;
 }
-// So few values of x that every workgroup of the product quantises them for itself.
-bool few_raw(int64_t N, int64_t K) { return few_tiles(N, (int)((K + KPAD - 1) / KPAD * KPAD)) && N * K <= 8192; }
+// So few values of x that every workgroup of the product quantises them for itself (one launch / two, us; x 16384 latents: 1 x
+// 768: 5.6 / 7.2, 8 x 1024: 7.1 / 7.1, 32 x 768: 10.3 / 7.0), in rows so short that the work is not split along them (1 x 4096: 17 / 10).
+bool few_raw(int64_t N, int64_t K) { return N * K <= 8192 && K <= 1024 && few_tiles(N, (int)((K + KPAD - 1) / KPAD * KPAD)); }
+
+int whole_lines(const void* out, int out_dtype, int64_t ldo) {
+  return (((uintptr_t)out | (uintptr_t)(ldo * (int64_t)dtype_size(out_dtype))) & 127) == 0;
+}
 
 template <typename XT, typename T>
 void launch_few(const LinearArgs& a, const XT* x, int64_t ldx, int64_t K, hipStream_t st) {
@@ -1035,35 +1011,35 @@ extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales,
   if (rc) return rc;
   CLT_CHECK_ARG(x_codes && x_scales, "clt_mxfp4_linear: null pointer");
   CLT_CHECK_ARG(aligned16(x_codes) && !((uintptr_t)x_scales & 3), "clt_mxfp4_linear: misaligned pointer");
-  LinearArgs a{x_codes, x_scales, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu};
-  if (few_tiles(N, a.kp)) {
-    if (out_dtype == CLT_BF16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, (hipStream_t)stream);
-    else launch_few<uint8_t, float>(a, nullptr, 0, K, (hipStream_t)stream);
-    CLT_CHECK_LAUNCH("clt_mxfp4_linear");
-    return CLT_OK;
+  LinearArgs a{x_codes, x_scales, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu, whole_lines(out, out_dtype, ldo)};
+  const auto st = (hipStream_t)stream;
+  const bool b16 = out_dtype == CLT_BF16;
+  const auto tiles = [&](int64_t m, int64_t n) { return (M + m - 1) / m * ((N + n - 1) / n); };
+  // Which kernel, with bf16 output, us (tokens x latents x columns; the kernels in their order below, - where one does not fit):
+  //   split / few:   33 x 16384 x 768: 5.6 / 8.0     8 x 43579 x 768: 6.0 / 6.6     8 x 98304 x 768: 11.0 / 9.5
+  //   split / tile:  200 x 6151 x 768: 7.6 / 7.9     950 x 2048 x 768: 7.7 / 7.1    128 x 16384 x 2048: 11.2 / 10.2
+  //   four waves a tile / one:  200 x 2048 x 4096: 7.1 / 9.7    509 x 2048 x 768: 7.6 / 5.5
+  //   few / tile:    33 x 43579 x 768: 9.7 / 9.9     33 x 98304 x 768: 12.9 / 14.4
+  //   big / tile:    2048 x 6151 x 2048: 24.7 / 28.6    509 x 16384 x 2048: 20.2 / 17.5    128 x 43579 x 2048: 21.9 / 16.3
+  const int64_t small = tiles(32, 32), mid = tiles(TM, TN), big = tiles(BM, BN);
+  CLT_UNSUPPORTED(mid < (1ll << 24), "clt_mxfp4_linear: fewer than 2^24 tiles of 128 x 128");  // (threads of a launch: 32 bits)
+  const bool few = few_tiles(N, a.kp);
+  if (small <= (N <= 64 ? 2048 : 1280) || (N <= 32 && !few)) {
+    const bool four = small <= 512;
+    const dim3 grid((unsigned)(four ? small : tiles(128, 32)));
+    const auto kernel = four ? (b16 ? mxfp4_split_kernel<bf16_t, 4> : mxfp4_split_kernel<float, 4>)
+                             : (b16 ? mxfp4_split_kernel<bf16_t, 1> : mxfp4_split_kernel<float, 1>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+  } else if (few) {
+    if (b16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, st);
+    else launch_few<uint8_t, float>(a, nullptr, 0, K, st);
+  } else if (big >= 192 && M > 128 && N > 128 && 256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
+    const auto kernel = b16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
+                            : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
+    hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t> : mxfp4_tile_kernel<float>), dim3((unsigned)mid), dim3(256), 0, st, a);
   }
-  const int64_t big = (M + BM - 1) / BM * ((N + BN - 1) / BN);
-  if (big >= 256 && big < (1ll << 31) && 256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
-    const auto kernel = out_dtype == CLT_BF16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
-                                              : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
-    hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, (hipStream_t)stream, a);
-    CLT_CHECK_LAUNCH("clt_mxfp4_linear");
-    return CLT_OK;
-  }
-  const int64_t tiles = (M + TM - 1) / TM * ((N + TN - 1) / TN);
-  if (N >= 16 && M >= 16 && tiles >= 64 && tiles < (1ll << 31)) {
-    if (out_dtype == CLT_BF16)
-      hipLaunchKernelGGL(mxfp4_tile_kernel<bf16_t>, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, a);
-    else
-      hipLaunchKernelGGL(mxfp4_tile_kernel<float>, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, a);
-    CLT_CHECK_LAUNCH("clt_mxfp4_linear");
-    return CLT_OK;
-  }
-  const dim3 grid((unsigned)((M + 31) / 32), (unsigned)((N + 31) / 32));
-  if (out_dtype == CLT_BF16)
-    hipLaunchKernelGGL(mxfp4_linear_kernel<bf16_t>, grid, dim3(64), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(mxfp4_linear_kernel<float>, grid, dim3(64), 0, (hipStream_t)stream, a);
   CLT_CHECK_LAUNCH("clt_mxfp4_linear");
   return CLT_OK;
 }
@@ -1081,7 +1057,7 @@ extern "C" int clt_mxfp4_linear_x(const void* x, int x_dtype, int64_t ldx, const
   CLT_CHECK_ARG(x && valid_dtype(x_dtype) && ldx >= 0 && !((uintptr_t)x & (dtype_size(x_dtype) - 1)),
                 "clt_mxfp4_linear_x: x is null or misaligned, or its dtype or stride is wrong");
   if (few_raw(N, K)) {
-    const LinearArgs a{nullptr, nullptr, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu};
+    const LinearArgs a{nullptr, nullptr, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu, whole_lines(out, out_dtype, ldo)};
     const hipStream_t st = (hipStream_t)stream;
     if (x_dtype == CLT_BF16) {
       if (out_dtype == CLT_BF16) launch_few<bf16_t, bf16_t>(a, (const bf16_t*)x, ldx, K, st);
