@@ -170,8 +170,9 @@ class AdamW(torch.optim.Optimizer):
     take the parameter's type as ``Adam``'s do.  ``state_bits=32``: float32 moments, whatever the parameters are.
     ``state_bits=8``: one byte per element and moment (the first moment and the square root of the second in e4m3, one
     power of two for 128 elements, stochastic rounding: hip_ops.adamw_step) for every tensor of at least
-    ``min_8bit_size`` elements; smaller ones keep float32 moments.  The reference's 8-bit choice is torchao's AdamW8bit
-    (trainer.py:155-164).  ``seed`` names the random bits: two runs with the same seed round alike.  Not capturable."""
+    ``min_8bit_size`` elements; smaller ones keep float32 moments.  (The reference's optimizer with 8-bit moments:
+    trainer.py:155-164.)  ``seed`` names the random bits: two runs with the same seed round alike.  One step count for all
+    parameters.  Not capturable."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
                  state_bits: int = 32, min_8bit_size: int = 4096, seed: int = 0):
@@ -212,10 +213,9 @@ class AdamW(torch.optim.Optimizer):
         calls = {}  # what one call has in common -> its tensors; groups usually differ in lr alone
         for group, ps in live:
             if ps:
-                key = (ps[0].device, group["betas"], group["eps"])
-                c = calls.setdefault(key, ([], [], [], [], [], []))
                 lr, wd = float(group["lr"]), float(group["weight_decay"])
                 for p in ps:
+                    c = calls.setdefault((p.device, tuple(group["betas"]), group["eps"]), ([], [], [], [], [], []))
                     m, v = self._moments(p)
                     for to, x in zip(c, (p, p.grad, m, v, lr, wd)):
                         to.append(x)

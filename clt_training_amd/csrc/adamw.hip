@@ -6,8 +6,9 @@
 // HBM-bound: per element 2 sizeof(p) + sizeof(g) bytes of parameter and gradient plus 16 (fp32 moments) or 4 + 4/128 (8-bit
 // moments).  Measured on four 98304 x 768 bf16 tables with bf16 gradients: 1.22 ms, 5.45 TB/s (fp32 moments), 0.53 ms, 5.7 TB/s
 // (8-bit moments); a large copy reaches 4.9 TB/s here.  The 8-bit path is near the vector units' limit, too: with the
-// stochastic rounding written out in integer arithmetic instead of the hardware's conversion it took 0.61 ms.  One launch takes up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device
-// memory, so nothing is uploaded, kept between calls or shared by two streams.  A workgroup owns one chunk of one tensor.
+// stochastic rounding written out in integer arithmetic instead of the hardware's conversion it took 0.61 ms.  One launch takes
+// up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device memory, so nothing is uploaded,
+// kept between calls or shared by two streams.  A workgroup owns one chunk of one tensor.
 //
 // 8-bit moments.  m and r = sqrt(v) are e4m3 (v itself spans twice the binades: a factor 2^17.8 between the largest and
 // the smallest gradient of a block is what r holds), scaled by 2^E for 128 consecutive elements: 16 lanes of 8 elements,
@@ -27,6 +28,7 @@ constexpr int MAX_TENSORS = 40;   // records in one launch's arguments (40 x 88 
 constexpr int VEC = 8;            // elements per lane and pass
 constexpr int CHUNK = 256 * VEC;  // elements per workgroup (twice as many: +3 %, four times: +9 % on 302 M elements)
 constexpr int BLOCK8 = 128;       // elements per scale
+constexpr int64_t MAX_CHUNKS = (1 << 24) - 1;  // workgroups of a launch (its threads are counted in 32 bits)
 
 struct Rec {
   char* p;
@@ -304,7 +306,6 @@ extern "C" int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, 
   CLT_CHECK_ARG(n_tensors >= 0 && (n_tensors == 0 || h_tensors), "clt_adamw_step: null pointer");
   CLT_CHECK_ARG(step >= 1, "clt_adamw_step: step is counted from 1");
   CLT_CHECK_ARG(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0, "clt_adamw_step: betas in [0, 1), eps >= 0");
-  int64_t total = 0;
   for (int i = 0; i < n_tensors; ++i) {
     const clt_adamw_tensor& t = h_tensors[i];
     CLT_CHECK_ARG(t.numel >= 0, "clt_adamw_step: tensor %d: negative size", i);
@@ -314,18 +315,17 @@ extern "C" int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, 
     const uintptr_t pm = dtype_size(t.p_dtype) - 1, gm = dtype_size(t.g_dtype) - 1, mm = t.m_scale ? 0 : 3;
     CLT_CHECK_ARG(!((uintptr_t)t.p & pm) && !((uintptr_t)t.g & gm) && !(((uintptr_t)t.m | (uintptr_t)t.v) & mm),
                   "clt_adamw_step: tensor %d: misaligned pointer", i);
-    total += t.numel;
+    CLT_UNSUPPORTED(t.numel <= MAX_CHUNKS * CHUNK, "clt_adamw_step: tensor %d: fewer than 2^35 - 2047 elements", i);
   }
-  CLT_CHECK_ARG(total < (1ll << 42), "clt_adamw_step: too many elements");
   const double bc1 = 1.0 - pow(b1, (double)step), bc2 = 1.0 - pow(b2, (double)step);
   Args a;
   a.c1 = (float)(1.0 - b1), a.b2 = (float)b2, a.c2 = (float)(1.0 - b2);
   a.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2)), a.eps = (float)eps;
   a.n = 0;
-  uint64_t chunks = 0;
+  int64_t chunks = 0;
   for (int i = 0; i <= n_tensors; ++i) {
-    const uint64_t mine = i < n_tensors ? ((uint64_t)h_tensors[i].numel + CHUNK - 1) / CHUNK : 0;
-    if (a.n && (i == n_tensors || a.n == MAX_TENSORS || chunks + mine >= (1ull << 31))) {
+    const int64_t mine = i < n_tensors ? (h_tensors[i].numel + CHUNK - 1) / CHUNK : 0;
+    if (a.n && (i == n_tensors || a.n == MAX_TENSORS || chunks + mine > MAX_CHUNKS)) {
       hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)chunks), dim3(256), 0, (hipStream_t)stream, a);
       CLT_CHECK_LAUNCH("clt_adamw_step");
       a.n = 0;

@@ -2,13 +2,14 @@
 // for torch tensors.  What a kernel of a few microseconds costs from Python is mostly this, so it is compiled; the library's
 // functions are handed over as addresses (bind), so that there is one loader (_lib.py) and one library.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <string>
-#include <unordered_set>
 #include <vector>
 
 #include "../../include/clt_mi355.h"
@@ -145,6 +146,8 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == N && out.size(1) == M && out.scalar_type() == odt &&
                           (M <= 1 || out.stride(1) == 1) && (N <= 1 || out.stride(0) >= M),
                       "mxfp4_linear: out must be [", N, ", ", M, "] ", odt, " with rows that do not overlap");
+    for (const Tensor* t : {&x_, packed ? &*x_scales : nullptr, &codes, &scales, bias_ ? &*bias_ : nullptr})
+      if (t) at::assert_no_overlap(out, *t);
   } else {
     out = at::empty({N, M}, codes.options().dtype(odt));
   }
@@ -168,6 +171,28 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
         "clt_mxfp4_linear_x");
   return out;
 }
+
+// Memory that a call writes must be no other argument's.
+struct Ranges {
+  struct Range {
+    uintptr_t first, end;
+    bool written;
+  };
+  std::vector<Range> all;
+  void add(const void* p, int64_t bytes, bool written) {
+    if (bytes) all.push_back({(uintptr_t)p, (uintptr_t)p + bytes, written});
+  }
+  bool clash() {
+    std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.first < b.first; });
+    uintptr_t any = 0, written = 0;  // where what has been seen ends
+    for (const Range& r : all) {
+      if (r.first < (r.written ? any : written)) return true;
+      any = std::max(any, r.end);
+      if (r.written) written = std::max(written, r.end);
+    }
+    return false;
+  }
+};
 
 // a number, or one per tensor
 std::vector<double> per_tensor(const py::object& v, size_t n, const char* name) {
@@ -197,11 +222,9 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                 "of the call, and every replay would repeat the same step");
   }
   std::vector<clt_adamw_tensor> table(n);
-  std::vector<Tensor> keep;  // contiguous copies outlive the launch, and so do the moments
-  std::unordered_set<const void*> seen;
-  size_t live = 0;
-  keep.reserve(4 * n);
-  seen.reserve(6 * n);
+  std::vector<Tensor> keep;  // contiguous copies outlive the launch
+  Ranges memory;
+  memory.all.reserve(6 * n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params[i];
     Tensor g = grads[i];
@@ -227,6 +250,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
         TORCH_CHECK_VALUE(c.sizes() == p.sizes() && c.is_contiguous() && c.device() == dev, "adamw_step: tensor ", i,
                           ": moments of the parameter's shape, contiguous, on ", dev);
         ptr[k] = c.mutable_data_ptr();
+        memory.add(ptr[k], 4 * numel, true);
       } else {
         const auto pair = o.cast<std::pair<Tensor, Tensor>>();
         const auto ct = pair.first.scalar_type(), st = pair.second.scalar_type();
@@ -239,18 +263,19 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                           "adamw_step: tensor ", i, ": one code per element and one scale per 128, contiguous, on ", dev);
         ptr[k] = pair.first.mutable_data_ptr();
         (k ? r.v_scale : r.m_scale) = static_cast<uint8_t*>(pair.second.mutable_data_ptr());
+        memory.add(ptr[k], numel, true);
+        memory.add(k ? r.v_scale : r.m_scale, (numel + 127) / 128, true);
       }
     }
     r.p = p.mutable_data_ptr(), r.g = g.const_data_ptr(), r.m = ptr[0], r.v = ptr[1];
     r.numel = numel, r.lr = lrs[i], r.weight_decay = wds[i];
     r.p_dtype = p.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
     r.g_dtype = g.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
-    if (numel) {
-      ++live;
-      seen.insert(r.p), seen.insert(r.m), seen.insert(r.v);
-    }
+    memory.add(r.p, numel * p.element_size(), true);
+    memory.add(r.g, numel * g.element_size(), false);
   }
-  TORCH_CHECK_VALUE(seen.size() == 3 * live, "adamw_step: a tensor is given twice (parameters and moments are updated in place)");
+  TORCH_CHECK_VALUE(!memory.clash(), "adamw_step: a tensor is given twice, or two share memory (parameters and moments are "
+                    "updated in place)");
   check(adamw_fn(table.data(), (int)n, betas.first, betas.second, eps, step, (uint32_t)seed, on.stream), "clt_adamw_step");
 }
 

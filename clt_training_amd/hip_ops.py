@@ -704,7 +704,8 @@ def mxfp4_linear(x, W: MXFP4Tensor, b: Optional[Tensor] = None, *, relu: bool = 
                  out: Optional[Tensor] = None) -> Tensor:
     """act(x @ W^T + b) on 4-bit operands with fp32 accumulation: ``x`` [N, K] is a tensor (its rows are quantised here) or
     an ``MXFP4Tensor``, ``W`` [M, K], ``b`` [M] or None; ``relu``: max(., 0), NaN stays NaN.  ``out_dtype`` defaults to the
-    dtype of ``x`` (float32 for an ``MXFP4Tensor``); ``out`` [N, M] may have any row stride."""
+    dtype of ``x`` (float32 for an ``MXFP4Tensor``); ``out`` [N, M] may have any row stride, but shares no memory with the
+    other arguments.  No autograd (``fused_encoder.fused_encoder`` with ``use_mxfp4`` has gradients)."""
     if not isinstance(W, MXFP4Tensor):
         raise TypeError("mxfp4_linear: W is an MXFP4Tensor (mxfp4_quantize)")
     if isinstance(x, MXFP4Tensor):
@@ -734,7 +735,8 @@ def encode_topk_mxfp4(x: Tensor, W, b: Optional[Tensor], k: int, out_dtype=None,
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay=0.01, seed: int = 0) -> None:
     """One AdamW step (decoupled weight decay) over lists of tensors, in place, with one launch for every 40 tensors.
-    params: float32 / bfloat16, contiguous, no two the same; grads: float32 / bfloat16 of the same shapes.
+    params: float32 / bfloat16, contiguous; grads: float32 / bfloat16 of the same shapes.  What is updated (parameters and
+    moments) shares no memory with another argument.
     ``exp_avgs[i]`` and ``exp_avg_sqs[i]`` are float32 tensors of the parameter's shape, or both are pairs (codes, scales):
     one byte per element (uint8 or float8_e4m3fn) and one byte per 128 elements (uint8 or float8_e8m0fnu) that hold the
     first moment and the SQUARE ROOT of the second in e4m3 times a power of two (all zero bytes: zero moments), rounded

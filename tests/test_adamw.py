@@ -182,6 +182,17 @@ def test_refusals_without_a_gpu():
     assert call() == -1
 
 
+def test_c_refusal_of_a_tensor_too_large_for_a_launch():
+    import ctypes as C
+
+    from clt_training_amd import _lib
+
+    rec = (_lib.AdamWTensor * 1)()
+    rec[0].p = rec[0].g = rec[0].m = rec[0].v = 4096
+    rec[0].numel = 2**35
+    assert _lib.load().clt_adamw_step(C.cast(rec, C.c_void_p), 1, 0.9, 0.99, 1e-8, 1, 0, None) == -2
+
+
 def test_trainer_takes_the_names_and_tp_refuses_them():
     from clt_training_amd import SparseCoderConfig, TrainConfig, Trainer
     from clt_training_amd.adam import AdamW
@@ -348,6 +359,24 @@ def test_more_than_2_to_32_elements():
         check_8bit(m[0][s], m[1][blk], m_new, lo, False)
         check_8bit(v[0][s], v[1][blk], r_new, hi, True)
     assert int((p != 0).sum()) <= sum(s.stop - s.start for s in spots)
+
+
+@pytest.mark.gpu
+def test_refuses_what_shares_memory():
+    from clt_training_amd import hip_ops as ops
+
+    p, g, m, v = make((300,), torch.float32, torch.float32, False, 1)
+    before = p.clone()
+    part = lambda t, k: t[k:k + 100]  # noqa: E731
+    with pytest.raises(ValueError, match="share memory"):  # (two parameters that overlap in part)
+        ops.adamw_step([part(p, 0), part(p, 99)], [part(g, 0), part(g, 100)], [part(m, 0), part(m, 100)], [part(v, 0), part(v, 100)], step=1)
+    with pytest.raises(ValueError, match="share memory"):  # (a gradient that is another tensor's moment)
+        ops.adamw_step([part(p, 0), part(p, 100)], [part(g, 0), part(m, 50)], [part(m, 0), part(m, 100)], [part(v, 0), part(v, 100)], step=1)
+    q, h, n, w = make((300,), torch.float32, torch.float32, True, 2)
+    with pytest.raises(ValueError, match="share memory"):  # (one array of scales for both moments)
+        ops.adamw_step([q], [h], [n], [(w[0], n[1])], step=1)
+    assert torch.equal(p, before)
+    ops.adamw_step([part(p, 0), part(p, 100)], [part(g, 0), part(g, 0)], [part(m, 0), part(m, 100)], [part(v, 0), part(v, 100)], step=1)  # (shared gradients are fine)
 
 
 @pytest.mark.gpu

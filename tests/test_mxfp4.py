@@ -96,6 +96,44 @@ def test_refusals_without_a_gpu():
     assert lib.clt_mxfp4_linear(p, p + 1, p, p, None, 0, 1, 8, 32, 0, p, 0, 8, None) == -1
 
 
+def test_c_refusals_of_sizes_and_workspace():
+    from clt_training_amd import _lib
+
+    lib = _lib.load()
+    p = 4096
+    assert lib.clt_mxfp4_quantize(p, 0, 32, 2**28, 128, p, p, None) == -1  # (more than a launch's threads can count)
+    assert lib.clt_mxfp4_dequantize(p, p, 2**28, 128, p, 0, None) == -1
+    x = lambda N, M, K, ws, size, a=p: lib.clt_mxfp4_linear_x(a, 0, K, p, p, None, 0, N, M, K, 0, p, 0, M, ws, size, None)  # noqa: E731
+    need = lib.clt_mxfp4_linear_x_workspace_bytes(70, 300)
+    assert need == 70 * 192 + 70 * 12
+    assert x(70, 8, 300, None, 0) == -4 and x(70, 8, 300, p, need - 1) == -4 and b"workspace" in lib.clt_last_error()
+    assert x(70, 8, 300, p + 4, need) == -1 and b"misaligned" in lib.clt_last_error()
+    assert x(70, 8, 300, p, need, None) == -1 and x(70, 8, 300, p, need, p + 2) == -1
+    assert x(70, 2**31, 300, p, need) == -2 and x(2**31, 8, 300, p, need) == -2 and x(2, 8, 2**24, p, need) == -2
+    assert lib.clt_mxfp4_linear_x_workspace_bytes(1, 768) == 0
+
+
+def test_large_product_keeps_its_registers(tmp_path):
+    """The waits of the 256 x 256 kernel count its stores and LDS transfers: a spilled register would be one more access
+    to memory than they know of.  The compiler's resource report must show no scratch for any of the product's kernels."""
+    import subprocess
+
+    from clt_training_amd.build import CSRC, FLAGS, HIPCC
+
+    out = subprocess.run([HIPCC, *FLAGS, "-Rpass-analysis=kernel-resource-usage", "-c", str(CSRC / "mxfp4.hip"), "-o", str(tmp_path / "o")],
+                         capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr[-2000:]
+    seen, name = {}, None
+    for line in out.stderr.splitlines():
+        if "Function Name:" in line:
+            name = line.split("Function Name:")[1].split()[0]
+        elif "ScratchSize" in line and name:
+            seen[name] = int(line.split("ScratchSize [bytes/lane]:")[1].split()[0])
+    for kernel, forms in (("mxfp4_big_kernel", 4), ("mxfp4_tile_kernel", 2), ("mxfp4_split_kernel", 4)):
+        found = {k: v for k, v in seen.items() if kernel in k}
+        assert len(found) == forms and not any(found.values()), found
+
+
 def test_fused_encoder_refuses_a_stray_quantised_weight():
     from clt_training_amd import hip_ops as ops
     from clt_training_amd.fused_encoder import fused_encoder
@@ -232,6 +270,121 @@ def test_linear_special_values():
             room = 256 * 2.0**-23 * (torch.nan_to_num(xq.dequantize().double()).abs() @ torch.nan_to_num(Wq.dequantize().double()).abs().t())
             assert ((y.double() - ref).abs() <= room)[ok].all()
             assert (y[3][:9] == 0).all() and (y[4:, 4] == 0).all()
+
+
+# Every way through the product: four waves a tile, one wave a tile (also where the tokens do not fit beside W), few tokens,
+# tiles of 128 x 128 and of 256 x 256.
+ROUTES = [(40, 300), (100, 5100), (20, 66001), (3, 70001), (50, 41003), (200, 8101), (520, 40001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [31, 128, 300, 512, 700])
+@pytest.mark.parametrize("N,M", ROUTES)
+def test_linear_every_route(N, M, K):
+    check_linear(N, M, K, torch.bfloat16, torch.bfloat16, torch.float32, True, N + K)
+    check_linear(N, M, K, torch.float32, torch.float32, torch.bfloat16, False, M + K, spread=3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M,K", [(2, 300, 20000), (20, 66001, 7000), (50, 41003, 2900), (300, 1000, 12000), (260, 50000, 2600)])
+def test_linear_long_rows(N, M, K):
+    check_linear(N, M, K, torch.bfloat16, torch.float32, torch.float32, False, N + K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M", ROUTES)
+def test_linear_special_values_every_route(N, M):
+    """As test_linear_special_values, with rows whose last 128 columns are followed by a row of NaN, and biases that are not
+    finite."""
+    from clt_training_amd import hip_ops as ops
+
+    x, W = matrix(N, 300, torch.float32, 1), matrix(M, 300, torch.float32, 2)
+    b = matrix(1, M, torch.float32, 3)[0]
+    x[1, 299], W[9, 3], W[M - 1, 200] = float("nan"), float("-inf"), float("nan")
+    b[0], b[1], b[2] = float("nan"), float("inf"), float("-inf")
+    xq, Wq = ops.mxfp4_quantize(x), ops.mxfp4_quantize(W)
+    xv, wv = xq.dequantize().double(), Wq.dequantize().double()
+    ref = xv @ wv.t() + b.double()
+    room = 300 * 2.0**-23 * (torch.nan_to_num(xv).abs() @ torch.nan_to_num(wv).abs().t()) + 2.0**-24 * ref.abs()
+    for relu in (False, True):
+        want = torch.where(ref < 0, 0, ref) if relu else ref
+        for given in (x, xq):
+            y = ops.mxfp4_linear(given, Wq, b, relu=relu)
+            assert torch.equal(torch.isnan(y), torch.isnan(want)) and int(torch.isnan(y).sum()) == M + 3 * (N - 1)
+            sure = torch.isfinite(want)
+            assert ((y.double() - want).abs() <= room)[sure].all() and torch.equal(y.double()[torch.isinf(want)], want[torch.isinf(want)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M", ROUTES)
+def test_linear_any_alignment_every_route(N, M):
+    """Rows of ``out`` at odd addresses and with gaps, bias and x at odd addresses: the same bits, and nothing beside them written."""
+    from clt_training_amd import hip_ops as ops
+
+    for dt in (torch.bfloat16, torch.float32):
+        xs = matrix(N, 303, torch.float32, 4)
+        b = matrix(1, M + 1, torch.bfloat16, 5)[0][1:]
+        Wq = ops.mxfp4_quantize(matrix(M, 300, torch.float32, 6))
+        want = ops.mxfp4_linear(xs[:, 1:301].contiguous(), Wq, b.clone(), relu=True, out_dtype=dt)
+        big = torch.full((N + 2, M + 9), 7.0, dtype=dt, device="cuda")
+        y = ops.mxfp4_linear(xs[:, 1:301], Wq, b, relu=True, out=big[1:N + 1, 3:3 + M])
+        assert torch.equal(y, want)
+        y.fill_(7)
+        assert (big == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M", ROUTES)
+def test_linear_two_graphs_and_two_streams(N, M):
+    """Two graphs of the same sizes, captured one after the other and replayed in turn with eager work between, and two streams at
+    once: no call shares anything with another."""
+    from clt_training_amd import hip_ops as ops
+
+    W = [ops.mxfp4_quantize(matrix(M, 300, torch.float32, 7 + i)) for i in range(2)]
+    x = [matrix(N, 300, torch.bfloat16, 9 + i) for i in range(2)]
+    eager = lambda i: ops.mxfp4_linear(x[i], W[i], relu=True)  # noqa: E731
+    eager(0), eager(1)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(eager(i))
+        graphs.append(g)
+    for seed in range(3):
+        for i in range(2):
+            x[i].copy_(matrix(N, 300, torch.bfloat16, 20 + 2 * seed + i))
+        want = [eager(0), eager(1)]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = eager(i)
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_linear_refuses_an_output_over_an_input():
+    from clt_training_amd import hip_ops as ops
+
+    x = matrix(64, 64, torch.float32, 1)
+    W = ops.mxfp4_quantize(matrix(64, 64, torch.float32, 2))
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.mxfp4_linear(x, W, out=x)
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.mxfp4_linear(x[:1], W, x[0], out=x[:1])
+    with pytest.raises(ValueError, match="overlap"):
+        ops.mxfp4_linear(x, W, out=x[:1].expand(64, 64))
+    assert ops.mxfp4_linear(x[:0], W).shape == (0, 64) and ops.mxfp4_linear(x, ops.mxfp4_quantize(x[:0])).shape == (64, 0)
 
 
 @pytest.mark.gpu
