@@ -204,17 +204,32 @@ std::vector<double> per_tensor(const py::object& v, size_t n, const char* name) 
   return std::vector<double>(n, v.cast<double>());
 }
 
-void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const py::sequence& first,
-                const py::sequence& second, int64_t step, const py::object& lr, std::pair<double, double> betas, double eps,
-                const py::object& weight_decay, int64_t seed) {
+// the items of a list, a tuple or what can be iterated
+struct Items {
+  py::object held;
+  explicit Items(const py::object& o) : held(py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "adamw_step: lists of tensors"))) {
+    if (!held) throw py::error_already_set();
+  }
+  size_t size() const { return PySequence_Fast_GET_SIZE(held.ptr()); }
+  PyObject* operator[](size_t i) const { return PySequence_Fast_GET_ITEM(held.ptr(), i); }
+  const Tensor& tensor(size_t i) const {
+    TORCH_CHECK_TYPE(THPVariable_Check((*this)[i]), "adamw_step: item ", i, " of the parameters or gradients is no tensor");
+    return THPVariable_Unpack((*this)[i]);
+  }
+};
+
+void adamw_step(const py::object& params_, const py::object& grads_, const py::object& first_, const py::object& second_,
+                int64_t step, const py::object& lr, std::pair<double, double> betas, double eps, const py::object& weight_decay,
+                int64_t seed) {
+  const Items params(params_), grads(grads_), first(first_), second(second_);
   const size_t n = params.size();
-  TORCH_CHECK_VALUE(grads.size() == n && first.size() == n && second.size() == n,
+  const auto lrs = per_tensor(lr, n, "lr"), wds = per_tensor(weight_decay, n, "weight_decay");
+  TORCH_CHECK_VALUE(params.size() == n && grads.size() == n && first.size() == n && second.size() == n,
                     "adamw_step: one gradient and two moments for every parameter");
   if (!n) return;
-  on_gpu(params[0]);
-  const auto dev = params[0].device();
-  const auto lrs = per_tensor(lr, n, "lr"), wds = per_tensor(weight_decay, n, "weight_decay");
-  const On on(params[0]);
+  on_gpu(params.tensor(0));
+  const auto dev = params.tensor(0).device();
+  const On on(params.tensor(0));
   {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     TORCH_CHECK(hipStreamIsCapturing((hipStream_t)on.stream, &status) == hipSuccess, "adamw_step: stream state");
@@ -226,8 +241,10 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   Ranges memory;
   memory.all.reserve(6 * n);
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& p = params[i];
-    Tensor g = grads[i];
+    const Tensor& p = params.tensor(i);
+    const bool dense = grads.tensor(i).is_contiguous();
+    if (!dense) keep.push_back(grads.tensor(i).contiguous());
+    const Tensor& g = dense ? grads.tensor(i) : keep.back();
     clt_adamw_tensor& r = table[i];
     r = {};
     TORCH_CHECK_TYPE((p.scalar_type() == at::kFloat || p.scalar_type() == at::kBFloat16) &&
@@ -235,16 +252,14 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                      "adamw_step: tensor ", i, ": only float32 / bfloat16, got ", p.scalar_type(), " and ", g.scalar_type());
     TORCH_CHECK_VALUE(p.device() == dev && g.device() == dev && g.sizes() == p.sizes() && p.is_contiguous(),
                       "adamw_step: tensor ", i, ": a contiguous parameter and a gradient of its shape, on ", dev);
-    if (!g.is_contiguous()) keep.push_back(g = g.contiguous());
     const int64_t numel = p.numel();
-    const py::object fo = first[i], so = second[i];
-    const bool eight = !THPVariable_Check(fo.ptr());
-    TORCH_CHECK_VALUE(eight != THPVariable_Check(so.ptr()), "adamw_step: tensor ", i, ": both moments in 32 bits or both in 8");
+    const bool eight = !THPVariable_Check(first[i]);
+    TORCH_CHECK_VALUE(eight != THPVariable_Check(second[i]), "adamw_step: tensor ", i, ": both moments in 32 bits or both in 8");
     void* ptr[2];
     for (int k = 0; k < 2; ++k) {
-      const py::object& o = k ? so : fo;
+      PyObject* o = k ? second[i] : first[i];
       if (!eight) {
-        const Tensor& c = THPVariable_Unpack(o.ptr());
+        const Tensor& c = THPVariable_Unpack(o);
         TORCH_CHECK_TYPE(c.scalar_type() == at::kFloat, "adamw_step: tensor ", i, ": moments are float32 or 8-bit pairs, got ",
                          c.scalar_type());
         TORCH_CHECK_VALUE(c.sizes() == p.sizes() && c.is_contiguous() && c.device() == dev, "adamw_step: tensor ", i,
@@ -252,7 +267,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
         ptr[k] = c.mutable_data_ptr();
         memory.add(ptr[k], 4 * numel, true);
       } else {
-        const auto pair = o.cast<std::pair<Tensor, Tensor>>();
+        const auto pair = py::handle(o).cast<std::pair<Tensor, Tensor>>();
         const auto ct = pair.first.scalar_type(), st = pair.second.scalar_type();
         TORCH_CHECK_TYPE((ct == at::kByte || ct == at::kFloat8_e4m3fn) && (st == at::kByte || st == at::kFloat8_e8m0fnu),
                          "adamw_step: tensor ", i, ": 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
