@@ -403,7 +403,7 @@ int clt_signsgd_step(const clt_adam_tensor* tensors, int n_tensors, const int32_
  *   128)]) for 128 consecutive elements: the least with max |.| 2^(127 - s) <= 448 (s = 0: all zero).  Rounded
  *   stochastically with 16 bits of a hash of (seed, position in h_tensors, step, element) per value; sqrt(v) > 0 stays > 0;
  *   NaN and infinite values become NaN.
- * step is 1-based.  Same arguments, same bits.                                                                     */
+ * step is 1-based.  Same arguments, same bits.  A tensor has fewer than 2^35 - 2047 elements.                       */
 typedef struct clt_adamw_tensor {
   void* p;
   const void* g;
@@ -429,7 +429,8 @@ int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, double b1, 
  *   a block that holds a NaN or an infinity has s = 255 and stands for NaN.  x [R, K] `x_dtype`, rows ldx elements apart.
  * dequantize: out [R, K] `out_dtype`, contiguous; bf16 holds every value exactly.
  * linear: out[n, m] = act(sum_k x[n, k] W[m, k] + bias[m]), fp32 accumulation, rounded once; act: ReLU (NaN stays NaN) or
- *   nothing; bias [M] `bias_dtype` or NULL; out rows ldo >= M elements apart.                                     */
+ *   nothing; bias [M] `bias_dtype` or NULL; out rows ldo >= M elements apart.
+ * Limits: R Kp < 2^35 - 2047 values in a quantise or dequantise call; N, M < 2^31 and K < 2^24 in a product.        */
 int clt_mxfp4_quantize(const void* x, int x_dtype, int64_t ldx, int64_t R, int64_t K, uint8_t* codes, uint8_t* scales,
                        clt_stream_t stream);
 int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t K, void* out, int out_dtype,
