@@ -3,6 +3,8 @@
 // functions are handed over as addresses (bind), so that there is one loader (_lib.py) and one library.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -70,6 +72,21 @@ struct On {
   }
 };
 
+// torch's allocation without its dispatcher (0.4 us less a tensor)
+Tensor empty(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(size, type, like.device(), std::nullopt);
+}
+// memory for the length of a call, on its stream (not kept: a captured graph then holds its own)
+struct Scratch {
+  void* p;
+  Scratch(size_t bytes, const On& on)
+      : p(bytes ? c10::hip::HIPCachingAllocator::raw_alloc_with_stream(bytes, (hipStream_t)on.stream) : nullptr) {}
+  Scratch(const Scratch&) = delete;
+  ~Scratch() {
+    if (p) c10::hip::HIPCachingAllocator::raw_delete(p);
+  }
+};
+
 // rows of unit stride (a copy if they have another)
 Tensor rows_of(const Tensor& x) { return x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x; }
 int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
@@ -92,8 +109,7 @@ std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x_) {
   TORCH_CHECK_VALUE(x_.size(1) >= 1, "mxfp4_quantize: no columns");
   const Tensor x = rows_of(x_);
   const int64_t R = x.size(0), K = x.size(1), kp = padded(K);
-  const auto opt = x.options().dtype(at::kByte);
-  Tensor codes = at::empty({R, kp / 2}, opt), scales = at::empty({R, kp / 32}, opt);
+  Tensor codes = empty({R, kp / 2}, at::kByte, x), scales = empty({R, kp / 32}, at::kByte, x);
   if (R) {
     const On on(x);
     check(quantize_fn(x.const_data_ptr(), dt, row_stride(x), R, K, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
@@ -107,7 +123,7 @@ Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols,
   const int dt = code_of(dtype);
   on_gpu(codes);
   check_codes(codes, scales, cols);
-  Tensor out = at::empty({codes.size(0), cols}, codes.options().dtype(dtype));
+  Tensor out = empty({codes.size(0), cols}, dtype, codes);
   if (out.numel()) {
     const On on(out);
     check(dequantize_fn(codes.const_data_ptr<uint8_t>(), scales.const_data_ptr<uint8_t>(), codes.size(0), cols,
@@ -149,7 +165,7 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     for (const Tensor* t : {&x_, packed ? &*x_scales : nullptr, &codes, &scales, bias_ ? &*bias_ : nullptr})
       if (t) at::assert_no_overlap(out, *t);
   } else {
-    out = at::empty({N, M}, codes.options().dtype(odt));
+    out = empty({N, M}, odt, codes);
   }
   if (N == 0 || M == 0) return out;
   const On on(out);
@@ -164,10 +180,9 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
   }
   const Tensor x = rows_of(x_);
   const size_t bytes = linear_x_bytes_fn(N, cols);
-  Tensor scratch;  // (from the allocator, not kept: a captured graph then holds its own)
-  if (bytes) scratch = at::empty({(int64_t)bytes}, codes.options());
+  const Scratch scratch(bytes, on);
   check(linear_x_fn(x.const_data_ptr(), xc, row_stride(x), wc, ws, bp, bc, N, M, cols, relu, out.mutable_data_ptr(), oc, ldo,
-                    bytes ? scratch.data_ptr() : nullptr, bytes, on.stream),
+                    scratch.p, bytes, on.stream),
         "clt_mxfp4_linear_x");
   return out;
 }
