@@ -158,7 +158,7 @@ __device__ __forceinline__ void store_row16(float* to, u32x4 w) {
   else *reinterpret_cast<u32x4_any4*>(to) = (u32x4_any4)w;
 }
 
-// Few tokens (at most 16 NT): bound by reading W, so W goes from memory to registers once and nothing else is in the way.  A wave
+// Few tokens (at most 16): bound by reading W, so W goes from memory to registers once and nothing else is in the way.  A wave
 // takes 16 rows of W at a time (v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, columns 32 (l / 16) .. + 31 of 128),
 // with the loads of the next 512 columns -- of the next rows, at a row's end -- in flight while it multiplies.  The tokens
 // lie in LDS, quantised there by every workgroup for itself when they are so few that this is cheaper than a launch (XT: float /
@@ -198,12 +198,12 @@ __device__ __forceinline__ void store_four(const LinearArgs& p, T* row, int64_t 
       if (m + i < p.M) row[m + i] = o.e[i];
   }
 }
-template <typename XT, typename T, int NT>
+template <typename XT, typename T>
 __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, const XT* __restrict__ x, int64_t ldx, int K) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int rowb = p.kp / 2, sb = p.kp / 32, pitch = rowb + 16, nks = p.kp / 128;
   const int N = (int)p.N;
-  char* xs = lds + NT * 16 * pitch;  // scales, sb bytes a row
+  char* xs = lds + 16 * pitch;  // scales, sb bytes a row
   if constexpr (sizeof(XT) == 1) {
     for (int i = threadIdx.x; i < N * (rowb / 16); i += 256) {
       const int row = i / (rowb / 16), c = i - row * (rowb / 16);
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, cons
   while (g < groups) {
     const int64_t m = g * 16 + 4 * q;  // this lane's four latents
     const f32x4 b = bias_four(p, m);
-    f32x4 acc[NT] = {};
+    f32x4 acc = {};
     const int64_t next = g + step;
     for (int c = 0; c < nch; ++c) {
       if (c + 1 < nch) load(g, c + 1, then);
@@ -253,37 +253,29 @@ __global__ __launch_bounds__(256) void mxfp4_few_kernel(const LinearArgs p, cons
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (4 * c + j >= nks) break;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const i32x4 xf = *reinterpret_cast<const i32x4*>(lds + (16 * t + r16) * pitch + 256 * c + 64 * j + 16 * q);
-          const uint32_t xsc = *reinterpret_cast<const uint32_t*>(xs + (16 * t + r16) * sb + 16 * c + 4 * j);
-          acc[t] = mfma4_16(__builtin_bit_cast(i32x4, now.w[j]), xf, acc[t], (int)(now.s[j] >> (8 * q)), (int)(xsc >> (8 * q)));
-        }
+        const i32x4 xf = *reinterpret_cast<const i32x4*>(lds + r16 * pitch + 256 * c + 64 * j + 16 * q);
+        const uint32_t xsc = *reinterpret_cast<const uint32_t*>(xs + r16 * sb + 16 * c + 4 * j);
+        acc = mfma4_16(__builtin_bit_cast(i32x4, now.w[j]), xf, acc, (int)(now.s[j] >> (8 * q)), (int)(xsc >> (8 * q)));
       }
       now = then;
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int n = 16 * t + r16;
-      if (n >= N) continue;
-      store_four(p, out + n * p.ldo, m, acc[t], b);
-    }
+    if (r16 < N) store_four(p, out + r16 * p.ldo, m, acc, b);
     g = next;
   }
 }
 
-// Middle-sized problems.  A workgroup of four waves computes 128 latents x 128 tokens, a wave 64 x 64 of them; two workgroups
-// share a CU, so that the waits, the first loads and the stores of one run beside the matrix instructions of the other.  Per
-// stage of 256 columns both operands come as whole lines of 128 bytes by LDS-DMA into a ring of two slots, one stage ahead; what
-// lies behind an array's last row reads as zeros.  Chunk c of a row lies at c ^ (row / 2 % 8): fragment reads (16 rows, one
-// chunk) hit every bank once.  The finished tile goes through the ring's LDS once, so that a store instruction writes rows of
-// 128 bytes and more.
-//   Bound by the time a stage takes from its fetch to its use (about 0.7 us a stage with one workgroup a CU) while tiles are
-// fewer than 512, then by LDS and the matrix instructions together.  512 tokens x 6151 x 4096: 18 us; 256 x 128 tiles with
-// stages of 128 columns took 28, three or four slots with one workgroup a CU 17 and up to 1.7 x these times where tiles are many;
-// a second barrier that lets a slot be refilled a step earlier saves 15 % where W comes from HBM for one row of tiles
-// (128 x 98304 x 768: 18 for 21 us) and costs 3 to 9 % elsewhere.
-constexpr int TM = 128, TN = 128, KS = 256, SLOT = (TM + TN) * (128 + 16);
+// Small and middle-sized problems.  A workgroup of four waves computes 64 B latents x 64 B tokens, a wave a quarter of them; four
+// (B = 1) or two workgroups share a CU, so that the waits, the first loads and the stores of one run beside the matrix
+// instructions of the others.  Per stage of 256 columns both operands come as whole lines of 128 bytes by LDS-DMA into a ring of
+// two slots, one stage ahead; what lies behind an array's last row reads as zeros.  Chunk c of a row lies at c ^ (row / 2 % 8):
+// fragment reads (16 rows, one chunk) hit every bank once.  The finished tile goes through the ring's LDS once, so that a store
+// instruction writes rows of 64 to 256 bytes.
+//   Bound by a stage's chain of fetch, fragment reads and matrix instructions (0.3 us with B = 1, 0.7 with B = 2) while there is
+// a workgroup or two a CU, then by LDS and the matrix instructions together: B = 2 reads LDS half as often per product.  950 tokens x
+// 2048 x 4096: 11.0 us with B = 1, 17.1 with B = 2 (256 x 128 tiles, stages of 128 columns: 26); 950 x 16384 x 768: 18.7, 16.9.
+//   Three or four slots with one workgroup a CU: the same at 512 x 6151 x 4096, up to 1.7 x the time where tiles are many.  A
+// second barrier that lets a slot be refilled a step earlier saves 15 % where W comes from HBM for one row of tiles (128 x 98304 x
+// 768: 18 for 21 us, B = 2) and costs 3 to 9 % elsewhere.
 constexpr int BPANEL = 16;  // latent tiles that run through all tokens together
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -407,73 +399,74 @@ __device__ __forceinline__ void lines_of(u32x4 (&c)[8]) {
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) {
-  static_assert(2 * 2 * SLOT <= 160 * 1024, "LDS of two workgroups");
+template <typename T, int B>
+__global__ __launch_bounds__(256, 4 / B) void mxfp4_tile_kernel(const LinearArgs p) {
+  constexpr int TS = 64 * B, WS = 32 * B, SLOT = 2 * TS * (128 + 16);  // side of a tile, of a wave's part; bytes of a stage
+  static_assert(4 / B * 2 * SLOT <= 160 * 1024, "LDS of 4 / B workgroups");
   __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5, wm = wave >> 1, wn = wave & 1;
 
   // ---- tile: an XCD (workgroup id % 8) owns a contiguous range of positions; a panel of latent tiles runs through all tokens
-  const int64_t nlt = (p.M + TM - 1) / TM, ntt = (p.N + TN - 1) / TN, ntiles = nlt * ntt;
+  const int64_t nlt = (p.M + TS - 1) / TS, ntt = (p.N + TS - 1) / TS, ntiles = nlt * ntt;
   const int64_t xg = blockIdx.x & 7, q = ntiles >> 3, rest = ntiles & 7;
   const int64_t pos = xg * q + min(xg, rest) + (blockIdx.x >> 3);
   const int64_t panel = pos / (ntt * BPANEL), in = pos - panel * ntt * BPANEL;
   const int64_t width = min((int64_t)BPANEL, nlt - panel * BPANEL);
-  const int64_t n0 = in / width * TN, m0 = (panel * BPANEL + in % width) * TM;
+  const int64_t n0 = in / width * TS, m0 = (panel * BPANEL + in % width) * TS;
 
-  // ---- loader: 64 rows a wave (waves 0, 1: W, 2, 3: x), eight pieces of eight rows and their scales
-  const int rowb = p.kp / 2, sb = p.kp / 32, nst = (p.kp + KS - 1) / KS;
-  const int64_t row0 = (wave < 2 ? m0 : n0) + 64 * (wave & 1), left = max((wave < 2 ? p.M : p.N) - row0, (int64_t)0);
+  // ---- loader: WS rows a wave (waves 0, 1: W, 2, 3: x), in pieces of eight rows, and their scales
+  const int rowb = p.kp / 2, sb = p.kp / 32, nst = (p.kp + 255) / 256;
+  const int64_t row0 = (wave < 2 ? m0 : n0) + WS * (wave & 1), left = max((wave < 2 ? p.M : p.N) - row0, (int64_t)0);
   const i32x4 cbuf = buffer_of((wave < 2 ? p.wc : p.xc) + row0 * rowb, left * rowb);
   const i32x4 sbuf = buffer_of((wave < 2 ? p.ws : p.xs) + row0 * sb, left * sb);
   const uint32_t chunk = ((lane & 7) ^ (lane >> 4)) << 4;
   const uint32_t even = (uint32_t)(lane >> 3) * rowb + chunk, odd = even - chunk + (chunk ^ 64);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + wave * 8192;
-  const uint32_t sc0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + (TM + TN) * 128 + wave * 1024;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + wave * (WS * 128);
+  const uint32_t sc0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + 2 * TS * 128 + wave * (WS * 16);
   auto fetch = [&](int s, int slot) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < WS / 8; ++i)
       dma16_buffer(cbuf, ((i & 1) ? odd : even) + (uint32_t)(128 * s + i * 8 * rowb), lds0 + slot * SLOT + i * 1024);
-    dma16_buffer(sbuf, (uint32_t)(lane * sb + 8 * s), sc0 + slot * SLOT);
+    dma16_lanes(sbuf, (uint32_t)(lane * sb + 8 * s), sc0 + slot * SLOT, -1, B == 1 ? 0 : -1);
   };
 
   // ---- multiplier
-  f32x16 acc[2][2] = {};  // [latents][tokens]; lane (r32, h): token r32, latents 8 g + 4 h + j
+  f32x16 acc[B][B] = {};  // [latents][tokens]; lane (r32, h): token r32, latents 8 g + 4 h + j
   const uint32_t at = r32 * 128 + ((h ^ (r32 >> 1 & 7)) << 4);
-  const uint32_t wat = wm * 8192 + at, xat = (2 + wn) * 8192 + at;
+  const uint32_t wat = wm * (WS * 128) + at, xat = (2 + wn) * (WS * 128) + at;
   fetch(0, 0);
   for (int s = 0; s < nst; ++s) {
     // stage s is there, and every wave is past stage s - 1
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (s + 1 < nst) fetch(s + 1, ~s & 1);
     const char* base = lds + (s & 1) * SLOT;
-    i32x4 w[2][4], x[2][4];
-    u32x2 sw[2], sx[2];
+    i32x4 w[B][4], x[B][4];
+    u32x2 sw[B], sx[B];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sw[i] = *reinterpret_cast<const u32x2*>(base + (TM + TN) * 128 + (wm * 64 + 32 * i + r32) * 16);
-      sx[i] = *reinterpret_cast<const u32x2*>(base + (TM + TN) * 128 + (TM + wn * 64 + 32 * i + r32) * 16);
+    for (int i = 0; i < B; ++i) {
+      sw[i] = *reinterpret_cast<const u32x2*>(base + 2 * TS * 128 + (wm * WS + 32 * i + r32) * 16);
+      sx[i] = *reinterpret_cast<const u32x2*>(base + 2 * TS * 128 + (TS + wn * WS + 32 * i + r32) * 16);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < B; ++i) {
         w[i][j] = *reinterpret_cast<const i32x4*>(base + i * 4096 + (wat ^ (32 * j)));
         x[i][j] = *reinterpret_cast<const i32x4*>(base + i * 4096 + (xat ^ (32 * j)));
       }
     const bool cut = 256 * s + 128 >= p.kp;  // (behind a row's last 128 columns stands the next row: counted 2^-254 times)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < B; ++i) {
       sw[i][1] = cut ? 0 : sw[i][1];
       sx[i][1] = cut ? 0 : sx[i][1];
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < B; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < B; ++k) {
           const int s1 = (int)(sw[i][j >> 1] >> (8 * h)), s2 = (int)(sx[k][j >> 1] >> (8 * h));
           acc[i][k] = j & 1 ? mfma4s<1>(w[i][j], x[k][j], acc[i][k], s1, s2) : mfma4s<0>(w[i][j], x[k][j], acc[i][k], s1, s2);
         }
@@ -481,9 +474,9 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
 
   // ---- epilogue: bias, ReLU, one rounding
   __syncthreads();  // (the ring is free)
-  constexpr int OPITCH = 64 * sizeof(T) + 16, VEC = 16 / sizeof(T), ROWL = 64 / VEC, ROWS = 64 / ROWL;
+  constexpr int OPITCH = WS * sizeof(T) + 16, VEC = 16 / sizeof(T), ROWL = WS / VEC, ROWS = 64 / ROWL;
   float* bias = reinterpret_cast<float*>(lds + 4 * 32 * OPITCH);
-  if (threadIdx.x < TM) {
+  if (threadIdx.x < TS) {
     const int64_t m = m0 + threadIdx.x;
     bias[threadIdx.x] = p.bias && m < p.M ? load_scalar(p.bias, p.bias_dtype, m) : 0.f;
   }
@@ -491,13 +484,13 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
   char* mine = lds + wave * 32 * OPITCH;
   T* out = reinterpret_cast<T*>(p.out);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < B; ++k) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < B; ++i) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int lat = i * 32 + 8 * g + 4 * h;
-        const float4 b = *reinterpret_cast<const float4*>(bias + wm * 64 + lat);
+        const float4 b = *reinterpret_cast<const float4*>(bias + wm * WS + lat);
         float v[4] = {acc[i][k][4 * g] + b.x, acc[i][k][4 * g + 1] + b.y, acc[i][k][4 * g + 2] + b.z, acc[i][k][4 * g + 3] + b.w};
         if (p.relu) {
 #pragma unroll
@@ -515,12 +508,12 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
     }
     asm volatile("" ::: "memory");  // (one wave, and a wave's LDS accesses are carried out in order)
     __builtin_amdgcn_wave_barrier();
-    const int64_t m = m0 + wm * 64 + (lane % ROWL) * VEC;
+    const int64_t m = m0 + wm * WS + (lane % ROWL) * VEC;
 #pragma unroll
     for (int i = 0; i < 32 / ROWS; ++i) {
       const int tok = ROWS * i + lane / ROWL;
       const u32x4 w = *reinterpret_cast<const u32x4*>(mine + tok * OPITCH + (lane % ROWL) * 16);
-      const int64_t n = n0 + wn * 64 + k * 32 + tok;
+      const int64_t n = n0 + wn * WS + k * 32 + tok;
       if (n >= p.N) continue;
       T* to = out + n * p.ldo + m;
       if (m + VEC <= p.M) {
@@ -538,32 +531,30 @@ __global__ __launch_bounds__(256, 2) void mxfp4_tile_kernel(const LinearArgs p) 
   }
 }
 
-// Problems of few tiles.  32 latents x 32 tokens by S of the four waves, each with a contiguous part of the columns; they add
-// up in LDS, in their order.  A wave works by itself: it fetches its rows 256 columns at a time, whole lines of 128 bytes, into
-// two slots of its own, so that no barrier stands in the loop.  (With fragments straight from memory, 16 lanes that are served
-// together read 16 lines: four times the accesses, and 11.8 us instead of 7.2 for 509 tokens x 884 x 4096.)
-// Bound by the loads' latency, from about four workgroups a CU on by their number of bytes (43 bytes a clock and CU).
+// Long rows, few tiles.  32 latents x 32 tokens by four waves, each with a contiguous quarter of the columns; they add up in LDS,
+// in their order.  A wave works by itself: it fetches its rows 256 columns at a time, whole lines of 128 bytes, into two slots of
+// its own, so that no barrier stands in the loop.  (With fragments straight from memory, 16 lanes that are served together read
+// 16 lines: four times the accesses, and 7.2 us instead of 4.7 for 128 tokens x 2048 x 4096.)  Bound by the loads' latency.
 constexpr int SB_ROW = 16;  // bytes of scales kept with a row and 256 columns (8 are its own)
-template <typename T, int S>
+template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_split_kernel(const LinearArgs p) {
-  constexpr int ROWS = 32, CODES = 2 * ROWS * 128, SLOT = CODES + 2 * ROWS * SB_ROW, PIECES = 2 * ROWS / 8 + 2;
+  constexpr int S = 4, ROWS = 32, CODES = 2 * ROWS * 128, SLOT = CODES + 2 * ROWS * SB_ROW, PIECES = 2 * ROWS / 8 + 2;
   constexpr int PITCH = ROWS + 8;  // of the sums, in floats
   static_assert(ROWS * PITCH * 4 <= 2 * SLOT && 8 * SLOT <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) char lds[8 * SLOT];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int turn = wave % S;
   char* own = lds + wave * 2 * SLOT;
   const uint32_t own0 = (uint32_t)(uintptr_t)(lds_ptr_t)own;
 
   // ---- tile: an XCD (workgroup id % 8) owns a contiguous range, tokens fastest: W comes to one L2 only
-  const int64_t nlt = (p.M + ROWS * (4 / S) - 1) / (ROWS * (4 / S)), ntt = (p.N + ROWS - 1) / ROWS, ntiles = nlt * ntt;
+  const int64_t nlt = (p.M + ROWS - 1) / ROWS, ntt = (p.N + ROWS - 1) / ROWS, ntiles = nlt * ntt;
   const int64_t xg = blockIdx.x & 7, share = ntiles >> 3, rest = ntiles & 7;
   const int64_t pos = xg * share + min(xg, rest) + (blockIdx.x >> 3);
-  const int64_t m0 = (pos / ntt * (4 / S) + wave / S) * ROWS, n0 = pos % ntt * ROWS;
+  const int64_t m0 = pos / ntt * ROWS, n0 = pos % ntt * ROWS;
 
   const int rowb = p.kp / 2, sb = p.kp / 32, nch = (p.kp + 255) / 256, per = (nch + S - 1) / S;
-  const int first = turn * per, stop = min(nch, first + per);
-  const int64_t mleft = max(p.M - m0, (int64_t)0), nleft = p.N - n0;
+  const int first = wave * per, stop = min(nch, first + per);
+  const int64_t mleft = p.M - m0, nleft = p.N - n0;
   const i32x4 wbuf = buffer_of(p.wc + m0 * rowb, mleft * rowb), xbuf = buffer_of(p.xc + n0 * rowb, nleft * rowb);
   const i32x4 wsbuf = buffer_of(p.ws + m0 * sb, mleft * sb), xsbuf = buffer_of(p.xs + n0 * sb, nleft * sb);
   auto none = [](i32x4 buf, bool on) {
@@ -606,7 +597,7 @@ __global__ __launch_bounds__(256) void mxfp4_split_kernel(const LinearArgs p) {
       acc = j & 1 ? mfma4s<1>(x[j], w[j], acc, s1, s2) : mfma4s<0>(x[j], w[j], acc, s1, s2);
     }
   };
-  if (first < stop && mleft) {
+  if (first < stop) {
     fetch(first, 0);
     fetch(first + 1, 1);
     for (int c = first; c < stop; ++c) {
@@ -621,14 +612,13 @@ __global__ __launch_bounds__(256) void mxfp4_split_kernel(const LinearArgs p) {
   __syncthreads();
   // four latents of a token per thread
   T* out = reinterpret_cast<T*>(p.out);
-  const char* parts = lds + (wave - turn) * 2 * SLOT;
   constexpr int QUADS = ROWS / 4;
 #pragma unroll
-  for (int e = 0; e < ROWS * QUADS / (64 * S); ++e) {
-    const int item = e * 64 * S + turn * 64 + lane, n = item / QUADS, m = item % QUADS * 4;
-    f32x4 v = *reinterpret_cast<const f32x4*>(parts + (n * PITCH + m) * 4);
+  for (int e = 0; e < ROWS * QUADS / 256; ++e) {
+    const int item = e * 256 + (int)threadIdx.x, n = item / QUADS, m = item % QUADS * 4;
+    f32x4 v = *reinterpret_cast<const f32x4*>(lds + (n * PITCH + m) * 4);
 #pragma unroll
-    for (int k = 1; k < S; ++k) v += *reinterpret_cast<const f32x4*>(parts + k * 2 * SLOT + (n * PITCH + m) * 4);
+    for (int k = 1; k < S; ++k) v += *reinterpret_cast<const f32x4*>(lds + k * 2 * SLOT + (n * PITCH + m) * 4);
     if (n < nleft && m < mleft) store_four(p, out + (n0 + n) * p.ldo, m0 + m, v, bias_four(p, m0 + m));
   }
 }
@@ -968,15 +958,11 @@ extern "C" int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
 namespace {
 
 constexpr int FEW_LDS = 64 * 1024;
-int few_lds(int nt, int kp) { return nt * 16 * (kp / 2 + 16 + kp / 32); }
-// 16, 32 or 64 tokens of kp columns in LDS (0: too many)
-int few_tiles(int64_t N, int kp) {
-  const int nt = N <= 16 ? 1 : N <= 32 ? 2 : N <= 64 ? 4 : 0;
-  return nt && few_lds(nt, kp) <= FEW_LDS ? nt : 0;
-}
+int few_lds(int kp) { return 16 * (kp / 2 + 16 + kp / 32); }
+bool few(int64_t N, int64_t K) { return N <= 16 && K < 16384 && few_lds((int)((K + KPAD - 1) / KPAD * KPAD)) <= FEW_LDS; }
 // So few values of x that every workgroup of the product quantises them for itself (one launch / two, us; x 16384 latents: 1 x
-// 768: 5.6 / 7.2, 8 x 1024: 7.1 / 7.1, 32 x 768: 10.3 / 7.0), in rows so short that the work is not split along them (1 x 4096: 17 / 10).
-bool few_raw(int64_t N, int64_t K) { return N * K <= 8192 && K <= 1024 && few_tiles(N, (int)((K + KPAD - 1) / KPAD * KPAD)); }
+// 768: 5.6 / 7.2, 8 x 1024: 7.1 / 7.1, 16 x 768: 7.4 / 7.0), in rows so short that reading W does not wait (1 x 4096: 17 / 10).
+bool few_raw(int64_t N, int64_t K) { return N * K <= 8192 && K <= 1024 && few(N, K); }
 
 int whole_lines(const void* out, int out_dtype, int64_t ldo) {
   return (((uintptr_t)out | (uintptr_t)(ldo * (int64_t)dtype_size(out_dtype))) & 127) == 0;
@@ -984,11 +970,9 @@ int whole_lines(const void* out, int out_dtype, int64_t ldo) {
 
 template <typename XT, typename T>
 void launch_few(const LinearArgs& a, const XT* x, int64_t ldx, int64_t K, hipStream_t st) {
-  const int nt = few_tiles(a.N, a.kp), lds = few_lds(nt, a.kp);
   const int64_t blocks = (a.M + 127) / 128;  // two groups of 16 rows and more a wave
   const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024));
-  const auto kernel = nt == 1 ? mxfp4_few_kernel<XT, T, 1> : nt == 2 ? mxfp4_few_kernel<XT, T, 2> : mxfp4_few_kernel<XT, T, 4>;
-  hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, x, ldx, (int)K);
+  hipLaunchKernelGGL((mxfp4_few_kernel<XT, T>), grid, dim3(256), few_lds(a.kp), st, a, x, ldx, (int)K);
 }
 
 int check_linear(const char* name, const void* w_codes, const void* w_scales, const void* bias, int bias_dtype, int64_t N,
@@ -1016,30 +1000,30 @@ extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales,
   const auto st = (hipStream_t)stream;
   const bool b16 = out_dtype == CLT_BF16;
   const auto tiles = [&](int64_t m, int64_t n) { return (M + m - 1) / m * ((N + n - 1) / n); };
-  // Which kernel, with bf16 output, us (tokens x latents x columns; the kernels in their order below, - where one does not fit):
-  //   split / few:   33 x 16384 x 768: 5.6 / 8.0     8 x 43579 x 768: 6.0 / 6.6     8 x 98304 x 768: 11.0 / 9.5
-  //   split / tile:  200 x 6151 x 768: 7.6 / 7.9     950 x 2048 x 768: 7.7 / 7.1    128 x 16384 x 2048: 11.2 / 10.2
-  //   four waves a tile / one:  200 x 2048 x 4096: 7.1 / 9.7    509 x 2048 x 768: 7.6 / 5.5
-  //   few / tile:    33 x 43579 x 768: 9.7 / 9.9     33 x 98304 x 768: 12.9 / 14.4
-  //   big / tile:    2048 x 6151 x 2048: 24.7 / 28.6    509 x 16384 x 2048: 20.2 / 17.5    128 x 43579 x 2048: 21.9 / 16.3
-  const int64_t small = tiles(32, 32), mid = tiles(TM, TN), big = tiles(BM, BN);
-  CLT_UNSUPPORTED(mid < (1ll << 24), "clt_mxfp4_linear: fewer than 2^24 tiles of 128 x 128");  // (threads of a launch: 32 bits)
-  const bool few = few_tiles(N, a.kp);
-  if (small <= (N <= 64 ? 2048 : 1280) || (N <= 32 && !few)) {
-    const bool four = small <= 512;
-    const dim3 grid((unsigned)(four ? small : tiles(128, 32)));
-    const auto kernel = four ? (b16 ? mxfp4_split_kernel<bf16_t, 4> : mxfp4_split_kernel<float, 4>)
-                             : (b16 ? mxfp4_split_kernel<bf16_t, 1> : mxfp4_split_kernel<float, 1>);
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
-  } else if (few) {
+  // Which kernel (tokens x latents x columns, bf16 output, us; - : does not fit):
+  //   few / 64 x 64:      1 x 98304 x 64: 5.1 / 6.0     1 x 98304 x 768: 8.9 / 10.1     1 x 43579 x 768: 6.4 / 5.4
+  //   split / 64 x 64:    128 x 2048 x 4096: 4.8 / 7.6     128 x 2048 x 2048: 4.2 / 5.5    200 x 1500 x 2048: 5.6 / 5.4
+  //   64 x 64 / 128 x 128:    950 x 6151 x 768: 9.9 / 10.9    509 x 6151 x 4096: 21.0 / 18.4    64 x 98304 x 768: 11.4 / 14.7
+  //                           64 x 131072 x 4096: 80 / 70
+  //   256 x 256 / the others: 950 x 16384 x 768: 13.8 / 16.9   2048 x 6151 x 2048: 23.7 / 26.7   2048 x 10000 x 768: 27.3 / 23.0
+  //                           200 x 43579 x 4096: 34 / 42
+  const int64_t t32 = tiles(32, 32), t64 = tiles(64, 64), t128 = tiles(128, 128), t256 = tiles(256, 256);
+  CLT_UNSUPPORTED(t128 < (1ll << 24), "clt_mxfp4_linear: fewer than 2^24 tiles of 128 x 128");  // (threads of a launch: 32 bits)
+  const int64_t stages = (a.kp + 255) / 256, rounds = (t256 + 255) / 256;  // (of one tile a CU)
+  if (few(N, K) && t64 > 1200) {
     if (b16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, st);
     else launch_few<uint8_t, float>(a, nullptr, 0, K, st);
-  } else if (big >= 192 && M > 128 && N > 128 && 256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
+  } else if (stages >= 4 && t32 <= 32 * stages && t32 <= 512) {
+    hipLaunchKernelGGL((b16 ? mxfp4_split_kernel<bf16_t> : mxfp4_split_kernel<float>), dim3((unsigned)t32), dim3(256), 0, st, a);
+  } else if (t256 >= 192 && M > 128 && N > 128 && (10 * t256 >= 7 * 256 * rounds || stages >= 10) &&
+             256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
     const auto kernel = b16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
                             : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
     hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, st, a);
+  } else if (t64 * (5 + stages) <= (N <= 64 ? 40000 : 15000)) {
+    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 1> : mxfp4_tile_kernel<float, 1>), dim3((unsigned)t64), dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t> : mxfp4_tile_kernel<float>), dim3((unsigned)mid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 2> : mxfp4_tile_kernel<float, 2>), dim3((unsigned)t128), dim3(256), 0, st, a);
   }
   CLT_CHECK_LAUNCH("clt_mxfp4_linear");
   return CLT_OK;

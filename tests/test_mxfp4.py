@@ -129,7 +129,7 @@ def test_large_product_keeps_its_registers(tmp_path):
             name = line.split("Function Name:")[1].split()[0]
         elif "ScratchSize" in line and name:
             seen[name] = int(line.split("ScratchSize [bytes/lane]:")[1].split()[0])
-    for kernel, forms in (("mxfp4_big_kernel", 4), ("mxfp4_tile_kernel", 2), ("mxfp4_split_kernel", 4)):
+    for kernel, forms in (("mxfp4_big_kernel", 4), ("mxfp4_tile_kernel", 4), ("mxfp4_split_kernel", 2)):
         found = {k: v for k, v in seen.items() if kernel in k}
         assert len(found) == forms and not any(found.values()), found
 
@@ -272,13 +272,13 @@ def test_linear_special_values():
             assert (y[3][:9] == 0).all() and (y[4:, 4] == 0).all()
 
 
-# Every way through the product: four waves a tile, one wave a tile (also where the tokens do not fit beside W), few tokens,
-# tiles of 128 x 128 and of 256 x 256.
-ROUTES = [(40, 300), (100, 5100), (20, 66001), (3, 70001), (50, 41003), (200, 8101), (520, 40001)]
+# Every way through the product: few tokens, tiles of 32 x 32 (long rows), 64 x 64, 128 x 128 and 256 x 256.
+ROUTES = [(40, 300), (100, 5100), (20, 66001), (3, 70001), (3, 90001), (50, 41003), (200, 8101), (500, 23001), (100, 100001), (520, 40001),
+          (2100, 30001)]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("K", [31, 128, 300, 512, 700])
+@pytest.mark.parametrize("K", [31, 128, 300, 512, 700, 1100])
 @pytest.mark.parametrize("N,M", ROUTES)
 def test_linear_every_route(N, M, K):
     check_linear(N, M, K, torch.bfloat16, torch.bfloat16, torch.float32, True, N + K)
