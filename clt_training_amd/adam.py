@@ -230,8 +230,13 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Moments keep the type they were saved in (the base class would cast them to the parameter's)."""
         sd = dict(state_dict)
-        step = sd.pop("clt_step", self._step)
         saved = sd.get("state", {})
+        step = sd.pop("clt_step", None)
+        if step is None:  # (a state that torch.optim wrote has a count for each parameter)
+            steps = {int(st["step"]) for st in saved.values() if "step" in st} or {self._step}
+            if len(steps) > 1:
+                raise ValueError(f"AdamW: one step count for all parameters, the saved state has {sorted(steps)}")
+            step = steps.pop()
         params = [p for g in self.param_groups for p in g["params"]]
         state = {}
         for i, st in saved.items():

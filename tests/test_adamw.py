@@ -228,6 +228,25 @@ def test_load_state_dict_keeps_types_and_refuses_what_does_not_fit():
             other.load_state_dict(opt.state_dict())
 
 
+def test_load_state_dict_of_torch():
+    from clt_training_amd.adam import AdamW
+
+    ps = [torch.nn.Parameter(torch.zeros(4, 5)), torch.nn.Parameter(torch.zeros(3))]
+    ref = torch.optim.AdamW(ps, lr=0.1, weight_decay=0.2)
+    for _ in range(3):
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        ref.step()
+    opt = AdamW(ps)
+    opt.load_state_dict(ref.state_dict())
+    assert opt._step == 3 and opt.param_groups[0]["weight_decay"] == 0.2
+    assert all(torch.equal(opt.state[p]["exp_avg_sq"], ref.state[p]["exp_avg_sq"]) for p in ps)
+    ref.state[ps[0]]["step"] += 1
+    with pytest.raises(ValueError, match="one step count"):
+        opt.load_state_dict(ref.state_dict())
+    assert opt._step == 3
+
+
 # ---------------------------------------------------------------------------------------------------------------- GPU
 SIZES = [(1,), (7,), (8,), (127,), (128,), (129,), (16, 8), (8191,), (8192,), (8193,), (33, 65), (257, 769)]
 
