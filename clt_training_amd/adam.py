@@ -231,6 +231,9 @@ class AdamW(torch.optim.Optimizer):
         """Moments keep the type they were saved in (the base class would cast them to the parameter's)."""
         sd = dict(state_dict)
         saved = sd.get("state", {})
+        for option in ("amsgrad", "maximize"):
+            if any(g.get(option) for g in sd.get("param_groups", ())):
+                raise ValueError(f"AdamW: the saved state was made with {option}=True")
         step = sd.pop("clt_step", None)
         if step is None:  # (a state that torch.optim wrote has a count for each parameter)
             steps = {int(st["step"]) for st in saved.values() if "step" in st} or {self._step}

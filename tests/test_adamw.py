@@ -245,6 +245,8 @@ def test_load_state_dict_of_torch():
     with pytest.raises(ValueError, match="one step count"):
         opt.load_state_dict(ref.state_dict())
     assert opt._step == 3
+    with pytest.raises(ValueError, match="maximize"):
+        opt.load_state_dict(torch.optim.AdamW(ps, maximize=True).state_dict())
 
 
 # ---------------------------------------------------------------------------------------------------------------- GPU
