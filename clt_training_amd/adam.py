@@ -171,8 +171,9 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits=8``: one byte per element and moment (the first moment and the square root of the second in e4m3, one
     power of two for 128 elements, stochastic rounding: hip_ops.adamw_step) for every tensor of at least
     ``min_8bit_size`` elements; smaller ones keep float32 moments.  (The reference's optimizer with 8-bit moments:
-    trainer.py:155-164.)  ``seed`` names the random bits: two runs with the same seed round alike.  One step count for all
-    parameters.  Not capturable."""
+    trainer.py:155-164.)  ``seed`` names the random bits: two runs with the same seed round alike.  Every parameter counts
+    the steps that updated it, as ``torch.optim.AdamW``'s do: one whose first gradient comes late starts with step 1's bias
+    correction.  Not capturable."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
                  state_bits: int = 32, min_8bit_size: int = 4096, seed: int = 0):
@@ -182,11 +183,15 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"invalid hyper-parameters: lr {float(lr)}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self.state_bits, self.min_8bit_size, self.seed = state_bits, min_8bit_size, seed
-        self._step = 0
+        self._step = 0  # calls of step() that updated something
+        self._steps = {}  # updates of each parameter
 
     def _moments(self, p):
         """The state of ``p`` as hip_ops.adamw_step takes it: (first, second)."""
         st = self.state[p]
+        if not st:
+            self._steps[p] = 0
+        self._steps.setdefault(p, self._step)  # (a state put there from outside)
         if not st:
             if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
                 for name in ("exp_avg", "rms"):
@@ -209,21 +214,27 @@ class AdamW(torch.optim.Optimizer):
             for p in ps:
                 if p.grad.is_sparse or not p.is_contiguous():
                     raise RuntimeError("AdamW needs dense gradients and contiguous parameters")
-        self._step += 1
-        calls = {}  # what one call has in common -> its tensors; groups usually differ in lr alone
+        calls = {}  # what one call has in common -> its tensors; groups usually differ in lr alone, and counts are alike
         for group, ps in live:
             if ps:
                 lr, wd = float(group["lr"]), float(group["weight_decay"])
                 for p in ps:
-                    c = calls.setdefault((p.device, tuple(group["betas"]), group["eps"]), ([], [], [], [], [], []))
                     m, v = self._moments(p)
+                    key = (p.device, tuple(group["betas"]), group["eps"], self._steps[p] + 1)
+                    c = calls.setdefault(key, ([], [], [], [], [], []))
                     for to, x in zip(c, (p, p.grad, m, v, lr, wd)):
                         to.append(x)
-        for (_, betas, eps), (ps, gs, ms, vs, lrs, wds) in calls.items():
-            adamw_step(ps, gs, ms, vs, step=self._step, lr=lrs, betas=betas, eps=eps, weight_decay=wds, seed=self.seed)
+        for (_, betas, eps, step), (ps, gs, ms, vs, lrs, wds) in calls.items():
+            adamw_step(ps, gs, ms, vs, step=step, lr=lrs, betas=betas, eps=eps, weight_decay=wds, seed=self.seed)
+            for p in ps:  # (a call that was refused counts for nothing)
+                self._steps[p] = step
+        self._step += bool(calls)
 
     def state_dict(self):
+        """As torch's (a parameter's count of updates is its state's ``step``), and ``clt_step``."""
         sd = super().state_dict()
+        params = [p for g in self.param_groups for p in g["params"]]
+        sd["state"] = {i: {**st, "step": torch.tensor(float(self._steps.get(params[i], self._step)))} if st else st for i, st in sd["state"].items()}
         sd["clt_step"] = self._step
         return sd
 
@@ -235,13 +246,14 @@ class AdamW(torch.optim.Optimizer):
             if any(g.get(option) for g in sd.get("param_groups", ())):
                 raise ValueError(f"AdamW: the saved state was made with {option}=True")
         step = sd.pop("clt_step", None)
-        if step is None:  # (a state that torch.optim wrote has a count for each parameter)
-            steps = {int(st["step"]) for st in saved.values() if "step" in st} or {self._step}
-            if len(steps) > 1:
-                raise ValueError(f"AdamW: one step count for all parameters, the saved state has {sorted(steps)}")
-            step = steps.pop()
+        counts = {i: int(st["step"]) for i, st in saved.items() if "step" in st}
+        if step is None:  # (written by torch.optim)
+            if len(set(counts.values())) > 1:
+                raise ValueError("AdamW: one step count for all parameters is expected of a state without 'clt_step', the saved one has "
+                                 f"{sorted(set(counts.values()))}; with state_dict['clt_step'] = {max(counts.values())} each keeps its own")
+            step = max(counts.values(), default=self._step)
         params = [p for g in self.param_groups for p in g["params"]]
-        state = {}
+        state, steps = {}, {}
         for i, st in saved.items():
             p, n = params[i], params[i].numel()
             want = ({"exp_avg": (torch.float32, n), "exp_avg_sq": (torch.float32, n)} if "exp_avg" in st else
@@ -250,9 +262,10 @@ class AdamW(torch.optim.Optimizer):
             for name, (dtype, size) in want.items():
                 if name not in st or st[name].numel() != size or (dtype == torch.uint8) != (st[name].dtype == torch.uint8):
                     raise ValueError(f"AdamW: the saved state of parameter {i} does not fit ({name})")
+            steps[p] = counts.get(i, step)  # (what an earlier version saved has one count for all)
             state[p] = {name: st[name].detach().to(device=p.device, dtype=dtype, copy=True).contiguous()
                         for name, (dtype, _) in want.items()}
         super().load_state_dict({**sd, "state": {}})
         self.state.clear()
         self.state.update(state)
-        self._step = step
+        self._step, self._steps = step, steps

@@ -245,6 +245,8 @@ class Trainer(EndToEnd, FitLoop):
         for i, opt in enumerate(self.optimizers):
             nested, step = ckpt.from_file_layout(torch.load(path / f"optimizer_{i}.pt", map_location=self.device,
                                                             weights_only=True))
+            if step is not None and hasattr(opt, "_step"):
+                nested["clt_step"] = step
             opt.load_state_dict(nested)  # (written by the reference or by save(): the same layout)
             if step is not None and hasattr(opt, "_step"):
                 opt._step = step
