@@ -401,8 +401,8 @@ int clt_signsgd_step(const clt_adam_tensor* tensors, int n_tensors, const int32_
  *   m_scale == v_scale == NULL: m and v fp32 [numel].
  *   else: m and v are e4m3 codes [numel] of m and sqrt(v), with one power of two 2^(s - 127) (one byte s, [ceil(numel /
  *   128)]) for 128 consecutive elements: the least with max |.| 2^(127 - s) <= 448 (s = 0: all zero).  Rounded
- *   stochastically with 16 bits of a hash of (seed, position in h_tensors, step, element) per value; sqrt(v) > 0 stays > 0;
- *   NaN and infinite values become NaN.
+ *   stochastically with 16 bits of a hash of (seed, position in h_tensors, step, element) per value; sqrt(v) > 0 stays > 0
+ *   (v is formed in fp32: below 2^-150 it is 0); NaN and infinite values become NaN.
  * step is 1-based.  Same arguments, same bits.  A tensor has fewer than 2^35 - 2047 elements.                       */
 typedef struct clt_adamw_tensor {
   void* p;

@@ -652,3 +652,44 @@ def test_late_parameters_against_torch():
         ropt.step()
     for p, q in zip(mine, ref):
         assert float((p.detach().cpu().double() - q.detach()).abs().max()) < 12 * 8 * U * 8
+
+
+@pytest.mark.gpu
+def test_subnormal_second_moments_32():
+    """v below 2^-126 has a root of its own, also with eps = 0.  b2 v is rounded to fp32's least steps, so the root's argument is
+    v as the call left it; from there on the module's 20 u of the update."""
+    from clt_training_amd import hip_ops as ops
+
+    n = 4096
+    gen = torch.Generator().manual_seed(1)
+    v = (torch.randint(2, 2**23, (n,), generator=gen) >> torch.randint(0, 21, (n,), generator=gen)).clamp(min=2).to(torch.int32).view(torch.float32)
+    assert float(v.min()) > 0 and float(v.max()) < 2.0**-126
+    v[1::4] = 2.0**-126 * (1 + torch.rand(v[1::4].shape, generator=gen))  # (normal neighbours)
+    m = torch.randn(n, generator=gen) * torch.sqrt(v.double()).float()
+    p, v, m = torch.zeros(n, device="cuda"), v.cuda(), m.cuda()
+    before = m.clone()
+    ops.adamw_step([p], [torch.zeros(n, device="cuda")], [m], [v], step=10, lr=1.0, betas=(B1, B2), eps=0.0, weight_decay=0.0)
+    assert bool((v > 0).all())
+    want = -1 / (1 - B1**10) * B1 * before.double() * math.sqrt(1 - B2**10) / torch.sqrt(v.double())
+    room = U * 20 * want.abs() + 3 * U * want.abs() + 2.0**-149  # (3 u: m', whose gradient is 0)
+    assert ((p.double() - want).abs() <= room).all()
+
+
+@pytest.mark.gpu
+def test_subnormal_second_moments_8():
+    """The stored root of a subnormal v: r > 0 stays > 0 wherever v = b2 r^2, formed in fp32, is."""
+    from clt_training_amd import hip_ops as ops
+
+    n = 126 * 128
+    codes = (torch.arange(n) % 126 + 1).to(torch.uint8)  # every positive value of e4m3
+    scale = torch.arange(126) % 14 + 127 - 80  # r^2 from below fp32's least step to normal numbers
+    r = codes.view(torch.float8_e4m3fn).float() * torch.exp2((scale - 127).double()).float().repeat_interleave(128)
+    v_new = r * r * torch.tensor(B2, dtype=torch.float32)
+    assert bool(((v_new > 0) & (v_new < 2.0**-126)).any()) and bool((v_new == 0).any()) and bool((v_new > 2.0**-126).any())
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    m = (torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(126, dtype=torch.uint8, device="cuda"))
+    second = (codes.cuda(), scale.to(torch.uint8).cuda())
+    ops.adamw_step([p], [g], [m], [second], step=4, betas=(B1, B2), seed=8)
+    _, hi = chances(8, 0, 4, torch.arange(n, device="cuda"))
+    check_8bit(*second, torch.sqrt(v_new.double()).cuda(), hi, True)
+    assert bool((p == 0).all())
