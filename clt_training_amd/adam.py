@@ -181,7 +181,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits is 8 or 32, got {state_bits}")
         if float(lr) < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError(f"invalid hyper-parameters: lr {float(lr)}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        # (the last entry is for torch.optim.Adam, which goes on from a saved state by it)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, decoupled_weight_decay=True))
         self.state_bits, self.min_8bit_size, self.seed = state_bits, min_8bit_size, seed
         self._step = 0  # calls of step() that updated something
         self._steps = {}  # updates of each parameter
@@ -266,6 +267,8 @@ class AdamW(torch.optim.Optimizer):
             state[p] = {name: st[name].detach().to(device=p.device, dtype=dtype, copy=True).contiguous()
                         for name, (dtype, _) in want.items()}
         super().load_state_dict({**sd, "state": {}})
+        for g in self.param_groups:
+            g["decoupled_weight_decay"] = True
         self.state.clear()
         self.state.update(state)
         self._step, self._steps = step, steps

@@ -7,6 +7,7 @@ p': the constant 1 - lr wd, its product and the sum: u (2 |p| + |p'|); the updat
 error of m' times s / denominator, and 20 u |D| for half of v's, the 1-ulp square root and reciprocal and five roundings.
 A bf16 parameter adds half a step of its type.  An 8-bit moment may differ from the oracle's only where the random bits
 decide within 2^-16 of a step (the value is off by at most 8 u, a step is at least 1/16 of it)."""
+import copy
 import math
 
 import pytest
@@ -328,6 +329,34 @@ def test_counts_of_torch_are_taken_over(monkeypatch):
     back = torch.optim.AdamW(ps)
     back.load_state_dict(opt.state_dict())
     assert [int(back.state[p]["step"]) for p in ps] == [4, 2]
+
+
+def test_saved_weight_decay_is_decoupled_for_torch():
+    """torch.optim.Adam goes on from a saved state, also from a checkpoint's file, as torch.optim.AdamW does; a state that an
+    earlier version saved with the other label is put right when it is loaded."""
+    from clt_training_amd import ckpt
+    from clt_training_amd.adam import AdamW
+
+    def ends(make, state):
+        p = torch.nn.Parameter(torch.linspace(1, 2, 6))
+        p.grad = torch.full((6,), 0.1)
+        opt = make([p])
+        opt.load_state_dict(copy.deepcopy(state))  # (torch steps on the tensors that it is given)
+        opt.step()
+        return p.detach()
+
+    q = torch.nn.Parameter(torch.zeros(6))
+    opt = AdamW([q], lr=1e-2, weight_decay=0.5)
+    m, v = opt._moments(q)
+    m.fill_(0.01), v.fill_(0.02)
+    opt._steps[q], opt._step = 4, 4
+    saved, step = ckpt.from_file_layout(ckpt.to_reference_layout(opt.state_dict(), opt._step))
+    for state in (saved, opt.state_dict()):
+        assert torch.equal(ends(torch.optim.Adam, state), ends(torch.optim.AdamW, state))
+    for g in saved["param_groups"]:
+        g["decoupled_weight_decay"] = False
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["decoupled_weight_decay"] is True and step == 4
 
 
 # ---------------------------------------------------------------------------------------------------------------- GPU
