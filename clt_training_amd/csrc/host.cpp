@@ -133,6 +133,27 @@ Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols,
   return out;
 }
 
+// Rows of equal length, equally far apart, in bytes.  (at::assert_no_overlap accepts what is not dense unseen.)
+struct Rows {
+  uintptr_t first;
+  int64_t count, pitch, width;
+  explicit Rows(const Tensor& t)  // (of unit stride in a row; a vector or what is contiguous is one row)
+      : first((uintptr_t)t.const_data_ptr()), count(1), pitch(0), width(t.numel() * t.element_size()) {
+    if (t.numel() && !t.is_contiguous()) count = t.size(0), pitch = t.stride(0) * t.element_size(), width = t.size(1) * t.element_size();
+  }
+  uintptr_t end() const { return first + (count - 1) * pitch + width; }
+  bool meets(const Rows& o) const {
+    if (!width || !o.width || first >= o.end() || o.first >= end()) return false;
+    for (int64_t n = 0; n < count; ++n) {
+      const uintptr_t low = first + n * pitch, high = low + width;
+      if (high <= o.first) continue;
+      const int64_t last = o.pitch ? std::min<int64_t>(o.count - 1, (high - 1 - o.first) / o.pitch) : 0;  // that begins below high
+      if (o.first + last * o.pitch + o.width > low) return true;
+    }
+    return false;
+  }
+};
+
 // x: a matrix, or codes with their scales
 Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& codes, const Tensor& scales, int64_t cols,
                     const OptTensor& bias_, bool relu, std::optional<at::ScalarType> dtype, const OptTensor& out_) {
@@ -152,7 +173,6 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     bias = bias_->contiguous();
   }
   const int xc = packed ? 0 : code_of(x_.scalar_type());
-  on_gpu(codes);
   same_device(codes, x_);
   if (bias_) same_device(codes, bias);
   Tensor out;
@@ -162,11 +182,15 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == N && out.size(1) == M && out.scalar_type() == odt &&
                           (M <= 1 || out.stride(1) == 1) && (N <= 1 || out.stride(0) >= M),
                       "mxfp4_linear: out must be [", N, ", ", M, "] ", odt, " with rows that do not overlap");
-    for (const Tensor* t : {&x_, packed ? &*x_scales : nullptr, &codes, &scales, bias_ ? &*bias_ : nullptr})
-      if (t) at::assert_no_overlap(out, *t);
-  } else {
-    out = empty({N, M}, odt, codes);
+    for (const Tensor* t : {&x_, packed ? &*x_scales : nullptr, &codes, &scales, bias_ ? &*bias_ : nullptr}) {
+      if (!t) continue;
+      at::assert_no_overlap(out, *t);
+      const bool in_place = t->dim() == 1 ? t->is_contiguous() : t->size(1) <= 1 || t->stride(1) == 1;  // (else a copy is read)
+      TORCH_CHECK(!in_place || !Rows(out).meets(Rows(*t)), "mxfp4_linear: out shares memory with another argument");
+    }
   }
+  on_gpu(codes);
+  if (!out_) out = empty({N, M}, odt, codes);
   if (N == 0 || M == 0) return out;
   const On on(out);
   const int64_t ldo = N > 1 ? out.stride(0) : M;

@@ -146,6 +146,45 @@ def test_fused_encoder_refuses_a_stray_quantised_weight():
         fused_encoder(x, torch.zeros(5, 128), b, 2, use_mxfp4=True, weight_mxfp4=W)
 
 
+def test_output_that_shares_memory_is_refused_whatever_its_strides():
+    """Random layouts of x, bias and an output with gaps in one buffer: refused exactly when a byte is common.  (On the CPU: a call
+    that passes the check is refused for that.)"""
+    import random
+
+    from clt_training_amd import hip_ops as ops
+
+    rng = random.Random(0)
+    seen = {True: 0, False: 0}
+    for _ in range(400):
+        N, M, K = rng.randint(1, 5), rng.randint(1, 6), rng.randint(1, 6)
+        buf = torch.zeros(150)
+        place = torch.arange(150)
+        view = lambda t, r, c, pitch, at: t.as_strided((r, c), (pitch, 1), at)  # noqa: E731
+        ox = (N, M, rng.randint(M, 12), rng.randint(0, 60))
+        xx = (N, K, rng.choice((0, K, ox[2], rng.randint(1, 12))), rng.randint(0, 60))
+        bx = (1, M, M, rng.randint(0, 100))
+        spot = [set(view(place, *a).flatten().tolist()) for a in (ox, xx, bx)]
+        common = bool(spot[0] & (spot[1] | spot[2]))
+        seen[common] += 1
+        W = ops.MXFP4Tensor(torch.zeros(M, 64, dtype=torch.uint8), torch.zeros(M, 4, dtype=torch.uint8), K)
+        with pytest.raises(RuntimeError, match="memory" if common else "no CPU fallback"):
+            ops.mxfp4_linear(view(buf, *xx), W, view(buf, *bx)[0], out=view(buf, *ox))
+    assert min(seen.values()) > 50
+    # the weight's codes and scales, and what is packed
+    room = torch.zeros(4096, dtype=torch.uint8)
+    codes, scales = room[1024:1024 + 8 * 64].view(8, 64), room[512:512 + 32].view(8, 4)
+    W, x = ops.MXFP4Tensor(codes, scales, 40), torch.zeros(3, 40)
+    other = ops.MXFP4Tensor(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.uint8), 40)
+    out = lambda at: room.view(torch.float32).as_strided((3, 8), (50, 1), at // 4)  # noqa: E731 (32 bytes every 200)
+    for given in ((x, W), (ops.MXFP4Tensor(codes[:3], scales[:3], 40), other)):
+        for at in (1024 - 32 - 400, 2048):
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                ops.mxfp4_linear(*given, out=out(at))
+        for at in (1024 - 4, 1024 - 200 + 160, 1024 - 400, 512 + 8 - 200):
+            with pytest.raises(RuntimeError, match="memory"):
+                ops.mxfp4_linear(*given, out=out(at))
+
+
 # ---------------------------------------------------------------------------------------------------------------- GPU
 def matrix(R, K, dtype, seed, spread=1.0):
     g = torch.Generator().manual_seed(seed)
@@ -552,3 +591,22 @@ def test_trainer_runs_with_4_bit_encoder(optimizer):
     enc = sae.encode(x)
     pre = ops.mxfp4_linear(x, ops.mxfp4_quantize(sae.encoder.weight.detach()), sae.encoder.bias.detach(), relu=True)
     assert torch.equal(enc.top_indices, ops.topk_rows(pre, 8)[1])
+
+
+@pytest.mark.gpu
+def test_linear_output_beside_its_inputs():
+    """An output with gaps between its rows: x or the bias in the gaps is fine, over them is refused."""
+    from clt_training_amd import hip_ops as ops
+
+    W = ops.mxfp4_quantize(matrix(64, 64, torch.float32, 2))
+    buf = torch.zeros(40, 160, device="cuda")
+    x = buf[:, :64]
+    x.copy_(matrix(40, 64, torch.float32, 1))
+    want = ops.mxfp4_linear(x.contiguous(), W)
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.mxfp4_linear(x, W, out=buf[:, 32:96])
+    with pytest.raises(RuntimeError, match="memory"):
+        ops.mxfp4_linear(want, W, buf[7, 70:134], out=buf[:, 96:])
+    assert torch.equal(ops.mxfp4_linear(x, W, out=buf[:, 64:128]), want)
+    half = buf[:, 0:128:2].clone()
+    assert torch.equal(ops.mxfp4_linear(buf[:, 0:128:2], W, out=buf[:, 64:128]), ops.mxfp4_linear(half, W))  # (a copy is read)
