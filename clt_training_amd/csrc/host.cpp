@@ -87,6 +87,11 @@ struct Scratch {
   }
 };
 
+// A tensor was written in place: autograd sees that a saved value is no longer there.  (Inference tensors have no count.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // rows of unit stride (a copy if they have another)
 Tensor rows_of(const Tensor& x) { return x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x; }
 int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
@@ -200,6 +205,7 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     check(linear_fn(x_.const_data_ptr<uint8_t>(), x_scales->const_data_ptr<uint8_t>(), wc, ws, bp, bc, N, M, cols, relu,
                     out.mutable_data_ptr(), oc, ldo, on.stream),
           "clt_mxfp4_linear");
+    if (out_) written(out);
     return out;
   }
   const Tensor x = rows_of(x_);
@@ -208,6 +214,7 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
   check(linear_x_fn(x.const_data_ptr(), xc, row_stride(x), wc, ws, bp, bc, N, M, cols, relu, out.mutable_data_ptr(), oc, ldo,
                     scratch.p, bytes, on.stream),
         "clt_mxfp4_linear_x");
+  if (out_) written(out);
   return out;
 }
 
@@ -331,6 +338,17 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   TORCH_CHECK_VALUE(!memory.clash(), "adamw_step: a tensor is given twice, or two share memory (parameters and moments are "
                     "updated in place)");
   check(adamw_fn(table.data(), (int)n, betas.first, betas.second, eps, step, (uint32_t)seed, on.stream), "clt_adamw_step");
+  for (size_t i = 0; i < n; ++i) {
+    written(params.tensor(i));
+    for (PyObject* o : {first[i], second[i]}) {
+      if (THPVariable_Check(o)) {
+        written(THPVariable_Unpack(o));
+      } else {
+        const auto pair = py::handle(o).cast<std::pair<Tensor, Tensor>>();
+        written(pair.first), written(pair.second);
+      }
+    }
+  }
 }
 
 }  // namespace

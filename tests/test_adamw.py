@@ -722,3 +722,28 @@ def test_subnormal_second_moments_8():
     _, hi = chances(8, 0, 4, torch.arange(n, device="cuda"))
     check_8bit(*second, torch.sqrt(v_new.double()).cuda(), hi, True)
     assert bool((p == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True])
+def test_autograd_sees_that_a_step_changed_its_tensors(eight):
+    """A parameter that changed between forward and backward is an error, as with torch's optimizers; a refused call changes
+    nothing; tensors of inference mode, which keep no count, are taken."""
+    from clt_training_amd import hip_ops as ops
+
+    p, g, m, v = make((256,), torch.float32, torch.float32, eight, 1)
+    moments = [*m, *v] if eight else [m, v]
+    x = torch.ones(256, device="cuda", requires_grad=True)
+    y = (x * p).sum()
+    versions = [t._version for t in (p, g, *moments)]
+    with pytest.raises(RuntimeError):
+        ops.adamw_step([p], [g], [m], [v], step=0)
+    assert [t._version for t in (p, g, *moments)] == versions
+    ops.adamw_step([p], [g], [m], [v], step=1)
+    assert [t._version - w for t, w in zip((p, g, *moments), versions)] == [1, 0] + [1] * len(moments)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        p, g, m, v = make((256,), torch.float32, torch.float32, eight, 1)
+        ops.adamw_step([p], [g], [m], [v], step=1)
+    ops.adamw_step([p], [g], [m], [v], step=2)

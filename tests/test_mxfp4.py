@@ -610,3 +610,20 @@ def test_linear_output_beside_its_inputs():
     assert torch.equal(ops.mxfp4_linear(x, W, out=buf[:, 64:128]), want)
     half = buf[:, 0:128:2].clone()
     assert torch.equal(ops.mxfp4_linear(buf[:, 0:128:2], W, out=buf[:, 64:128]), ops.mxfp4_linear(half, W))  # (a copy is read)
+
+
+@pytest.mark.gpu
+def test_autograd_sees_that_an_output_was_written():
+    from clt_training_amd import hip_ops as ops
+
+    W = ops.mxfp4_quantize(matrix(64, 64, torch.float32, 2))
+    a = matrix(40, 64, torch.float32, 1)
+    for given in (a, ops.mxfp4_quantize(a)):
+        buf = torch.zeros(40, 64, device="cuda")
+        y = (torch.ones(40, 64, device="cuda", requires_grad=True) * buf).sum()
+        ops.mxfp4_linear(given, W, out=buf)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        buf = torch.zeros(40, 64, device="cuda")
+    assert torch.equal(ops.mxfp4_linear(a, W, out=buf), ops.mxfp4_linear(a, W))
