@@ -187,6 +187,10 @@ class AdamW(torch.optim.Optimizer):
         self._step = 0  # calls of step() that updated something
         self._steps = {}  # updates of each parameter
 
+    def __getstate__(self):  # (of a copy or a pickle: torch's has the groups and the state alone)
+        own = ("state_bits", "min_8bit_size", "seed", "_step", "_steps")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in own}}
+
     def _moments(self, p):
         """The state of ``p`` as hip_ops.adamw_step takes it: (first, second)."""
         st = self.state[p]

@@ -359,6 +359,30 @@ def test_saved_weight_decay_is_decoupled_for_torch():
     assert opt.param_groups[0]["decoupled_weight_decay"] is True and step == 4
 
 
+def test_copies_go_on_where_the_optimizer_stands(monkeypatch):
+    import pickle
+
+    from clt_training_amd import adam
+
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in (5000, 3)]
+    opt = adam.AdamW(ps, lr=0.1, state_bits=8, seed=6)
+    recorded(monkeypatch)
+    for grads in ((1, 0), (1, 1)):
+        for p, on in zip(ps, grads):
+            p.grad = torch.ones_like(p) if on else None
+        opt.step()
+    opt.state[ps[0]]["rms_codes"].fill_(3)
+    for new in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        qs = [q for g in new.param_groups for q in g["params"]]
+        assert not any(p is q for p, q in zip(ps, qs)) and bool((new.state[qs[0]]["rms_codes"] == 3).all())
+        for q in qs:
+            q.grad = torch.ones_like(q)
+        calls = []
+        monkeypatch.setattr(adam, "adamw_step", lambda c, g, m, v, *, step, lr, seed, **kw: calls.append((len(c), type(m[0]) is tuple, step, lr[0], seed)))
+        new.step()
+        assert sorted(calls) == [(1, False, 2, 0.1, 6), (1, True, 3, 0.1, 6)] and new._step == 3 and opt._step == 2
+
+
 # ---------------------------------------------------------------------------------------------------------------- GPU
 SIZES = [(1,), (7,), (8,), (127,), (128,), (129,), (16, 8), (8191,), (8192,), (8193,), (33, 65), (257, 769)]
 
