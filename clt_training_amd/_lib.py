@@ -110,6 +110,7 @@ SIGNATURES = {
     "clt_mxfp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
     "clt_mxfp4_dequantize": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     "clt_mxfp4_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _i64, _vp]),
+    "clt_mxfp4_linear_route": (C.c_char_p, [_i64, _i64, _i64, _i32, _i64]),
     "clt_mxfp4_linear_x_workspace_bytes": (_sz, [_i64, _i64]),
     "clt_mxfp4_linear_x": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _i64, _vp, _sz, _vp]),
 }

@@ -968,6 +968,26 @@ int whole_lines(const void* out, int out_dtype, int64_t ldo) {
   return (((uintptr_t)out | (uintptr_t)(ldo * (int64_t)dtype_size(out_dtype))) & 127) == 0;
 }
 
+// Which kernel takes a problem of codes (tokens x latents x columns, bf16 output, us):
+//   few / 64 x 64:      1 x 98304 x 64: 5.1 / 6.0     1 x 98304 x 768: 8.9 / 10.1     1 x 43579 x 768: 6.4 / 5.4
+//   split / 64 x 64:    128 x 2048 x 4096: 4.8 / 7.6     128 x 2048 x 2048: 4.2 / 5.5    200 x 1500 x 2048: 5.6 / 5.4
+//   64 x 64 / 128 x 128:    950 x 6151 x 768: 9.9 / 10.9    509 x 6151 x 4096: 21.0 / 18.4    64 x 98304 x 768: 11.4 / 14.7
+//                           64 x 131072 x 4096: 80 / 70
+//   256 x 256 / the others: 950 x 16384 x 768: 13.8 / 16.9   2048 x 6151 x 2048: 23.7 / 26.7   2048 x 10000 x 768: 27.3 / 23.0
+//                           200 x 43579 x 4096: 34 / 42
+enum Route { FEW, SPLIT, TILE64, TILE128, BIG };
+int64_t tiles(int64_t M, int64_t N, int64_t side) { return (M + side - 1) / side * ((N + side - 1) / side); }
+Route route_of(int64_t N, int64_t M, int64_t K, int out_dtype, int64_t ldo) {
+  const int64_t t32 = tiles(M, N, 32), t64 = tiles(M, N, 64), t256 = tiles(M, N, 256);
+  const int64_t stages = (padded(K) + 255) / 256, rounds = (t256 + 255) / 256;  // (of one tile a CU)
+  if (few(N, K) && t64 > 1200) return FEW;
+  if (stages >= 4 && t32 <= 32 * stages && t32 <= 512) return SPLIT;
+  if (t256 >= 192 && M > 128 && N > 128 && (10 * t256 >= 7 * 256 * rounds || stages >= 10) &&
+      256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31))
+    return BIG;
+  return t64 * (5 + stages) <= (N <= 64 ? 40000 : 15000) ? TILE64 : TILE128;
+}
+
 template <typename XT, typename T>
 void launch_few(const LinearArgs& a, const XT* x, int64_t ldx, int64_t K, hipStream_t st) {
   const int64_t blocks = (a.M + 127) / 128;  // two groups of 16 rows and more a wave
@@ -999,34 +1019,37 @@ extern "C" int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales,
   LinearArgs a{x_codes, x_scales, w_codes, w_scales, bias, out, N, M, ldo, (int)padded(K), bias_dtype, relu, whole_lines(out, out_dtype, ldo)};
   const auto st = (hipStream_t)stream;
   const bool b16 = out_dtype == CLT_BF16;
-  const auto tiles = [&](int64_t m, int64_t n) { return (M + m - 1) / m * ((N + n - 1) / n); };
-  // Which kernel (tokens x latents x columns, bf16 output, us; - : does not fit):
-  //   few / 64 x 64:      1 x 98304 x 64: 5.1 / 6.0     1 x 98304 x 768: 8.9 / 10.1     1 x 43579 x 768: 6.4 / 5.4
-  //   split / 64 x 64:    128 x 2048 x 4096: 4.8 / 7.6     128 x 2048 x 2048: 4.2 / 5.5    200 x 1500 x 2048: 5.6 / 5.4
-  //   64 x 64 / 128 x 128:    950 x 6151 x 768: 9.9 / 10.9    509 x 6151 x 4096: 21.0 / 18.4    64 x 98304 x 768: 11.4 / 14.7
-  //                           64 x 131072 x 4096: 80 / 70
-  //   256 x 256 / the others: 950 x 16384 x 768: 13.8 / 16.9   2048 x 6151 x 2048: 23.7 / 26.7   2048 x 10000 x 768: 27.3 / 23.0
-  //                           200 x 43579 x 4096: 34 / 42
-  const int64_t t32 = tiles(32, 32), t64 = tiles(64, 64), t128 = tiles(128, 128), t256 = tiles(256, 256);
-  CLT_UNSUPPORTED(t128 < (1ll << 24), "clt_mxfp4_linear: fewer than 2^24 tiles of 128 x 128");  // (threads of a launch: 32 bits)
-  const int64_t stages = (a.kp + 255) / 256, rounds = (t256 + 255) / 256;  // (of one tile a CU)
-  if (few(N, K) && t64 > 1200) {
-    if (b16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, st);
-    else launch_few<uint8_t, float>(a, nullptr, 0, K, st);
-  } else if (stages >= 4 && t32 <= 32 * stages && t32 <= 512) {
-    hipLaunchKernelGGL((b16 ? mxfp4_split_kernel<bf16_t> : mxfp4_split_kernel<float>), dim3((unsigned)t32), dim3(256), 0, st, a);
-  } else if (t256 >= 192 && M > 128 && N > 128 && (10 * t256 >= 7 * 256 * rounds || stages >= 10) &&
-             256 * ldo * (int64_t)dtype_size(out_dtype) < (1ll << 31)) {
-    const auto kernel = b16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
-                            : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
-    hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, st, a);
-  } else if (t64 * (5 + stages) <= (N <= 64 ? 40000 : 15000)) {
-    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 1> : mxfp4_tile_kernel<float, 1>), dim3((unsigned)t64), dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 2> : mxfp4_tile_kernel<float, 2>), dim3((unsigned)t128), dim3(256), 0, st, a);
+  CLT_UNSUPPORTED(tiles(M, N, 128) < (1ll << 24), "clt_mxfp4_linear: fewer than 2^24 tiles of 128 x 128");  // (threads of a launch: 32 bits)
+  switch (route_of(N, M, K, out_dtype, ldo)) {
+    case FEW:
+      if (b16) launch_few<uint8_t, bf16_t>(a, nullptr, 0, K, st);
+      else launch_few<uint8_t, float>(a, nullptr, 0, K, st);
+      break;
+    case SPLIT:
+      hipLaunchKernelGGL((b16 ? mxfp4_split_kernel<bf16_t> : mxfp4_split_kernel<float>), dim3((unsigned)tiles(M, N, 32)), dim3(256), 0, st, a);
+      break;
+    case BIG: {
+      const auto kernel = b16 ? (relu ? mxfp4_big_kernel<bf16_t, true> : mxfp4_big_kernel<bf16_t, false>)
+                              : (relu ? mxfp4_big_kernel<float, true> : mxfp4_big_kernel<float, false>);
+      hipLaunchKernelGGL(kernel, dim3(256), dim3(512), 0, st, a);
+      break;
+    }
+    case TILE64:
+      hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 1> : mxfp4_tile_kernel<float, 1>), dim3((unsigned)tiles(M, N, 64)), dim3(256), 0, st, a);
+      break;
+    case TILE128:
+      hipLaunchKernelGGL((b16 ? mxfp4_tile_kernel<bf16_t, 2> : mxfp4_tile_kernel<float, 2>), dim3((unsigned)tiles(M, N, 128)), dim3(256), 0, st, a);
+      break;
   }
   CLT_CHECK_LAUNCH("clt_mxfp4_linear");
   return CLT_OK;
+}
+
+extern "C" const char* clt_mxfp4_linear_route(int64_t N, int64_t M, int64_t K, int out_dtype, int64_t ldo) {
+  static const char* const names[] = {"few", "split", "64 x 64", "128 x 128", "256 x 256"};
+  const bool taken = N > 0 && M > 0 && K > 0 && ldo >= M && valid_dtype(out_dtype) && N < (1ll << 31) && M < (1ll << 31) &&
+                     K < (1ll << 24) && tiles(M, N, 128) < (1ll << 24);
+  return taken ? names[route_of(N, M, K, out_dtype, ldo)] : "";
 }
 
 extern "C" size_t clt_mxfp4_linear_x_workspace_bytes(int64_t N, int64_t K) {

@@ -430,7 +430,8 @@ int clt_adamw_step(const clt_adamw_tensor* h_tensors, int n_tensors, double b1, 
  * dequantize: out [R, K] `out_dtype`, contiguous; bf16 holds every value exactly.
  * linear: out[n, m] = act(sum_k x[n, k] W[m, k] + bias[m]), fp32 accumulation, rounded once; act: ReLU (NaN stays NaN) or
  *   nothing; bias [M] `bias_dtype` or NULL; out rows ldo >= M elements apart.
- * Limits: R Kp < 2^35 - 2047 values in a quantise or dequantise call; N, M < 2^31 and K < 2^24 in a product.        */
+ * Limits: R Kp < 2^35 - 2047 values in a quantise or dequantise call; N, M < 2^31, K < 2^24 and fewer than 2^24 tiles
+ *   of 128 x 128 outputs in a product.                                                                               */
 int clt_mxfp4_quantize(const void* x, int x_dtype, int64_t ldx, int64_t R, int64_t K, uint8_t* codes, uint8_t* scales,
                        clt_stream_t stream);
 int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t K, void* out, int out_dtype,
@@ -438,6 +439,9 @@ int clt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R,
 int clt_mxfp4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
                      const void* bias, int bias_dtype, int64_t N, int64_t M, int64_t K, int relu, void* out, int out_dtype,
                      int64_t ldo, clt_stream_t stream);
+/* The kernel that clt_mxfp4_linear launches for these sizes: "few", "split", "64 x 64", "128 x 128" or "256 x 256" ("" for
+ * sizes that it refuses).  For tests and profiles; nothing is launched. */
+const char* clt_mxfp4_linear_route(int64_t N, int64_t M, int64_t K, int out_dtype, int64_t ldo);
 
 /* quantize and linear in one call, for x [N, K] `x_dtype` with rows ldx elements apart: the codes of x go through
  * `workspace` (clt_mxfp4_linear_x_workspace_bytes(N, K) bytes, 16-byte aligned, nothing in it outlives the call), or, for

@@ -185,6 +185,30 @@ def test_output_that_shares_memory_is_refused_whatever_its_strides():
                 ops.mxfp4_linear(*given, out=out(at))
 
 
+def route(N, M, K, dtype=torch.bfloat16, ldo=None):
+    from clt_training_amd import _lib
+
+    return _lib.load().clt_mxfp4_linear_route(N, M, K, 0 if dtype == torch.float32 else 1, M if ldo is None else ldo).decode()
+
+
+def test_routes_that_the_cases_below_are_meant_for():
+    """Every kernel has its cases; what the large kernel's cases need to reach its whole-line stores holds for them."""
+    every = {"few", "split", "64 x 64", "128 x 128", "256 x 256"}
+    for K, cases in ((300, ROUTES), (1100, LONG_ROUTES[:-1]), (1900, LONG_ROUTES[-1:])):
+        found = {route(N, M, K) for N, M in cases}
+        assert found == {300: every - {"split"}, 1100: every, 1900: {"split"}}[K], (K, found)
+    for N, M in WHOLE_LINES:
+        for K in (64, 300, 512, 700):
+            for dtype, size in ((torch.float32, 4), (torch.bfloat16, 2)):
+                assert route(N, M, K, dtype) == "256 x 256" and M * size % 128 == 0
+                assert -(-N // 256) * -(-M // 256) > 3 * 256  # (several tiles for every workgroup)
+    from clt_training_amd import _lib
+
+    for sizes in ((0, 8, 32), (1, 0, 32), (1, 8, 0), (1, 8, 32, torch.float32, 7), (2**31, 8, 32), (8, 8, 2**24), (2**20, 2**20, 32)):
+        assert route(*sizes) == ""
+    assert _lib.load().clt_mxfp4_linear_route(1, 8, 32, 9, 8) == b""
+
+
 # ---------------------------------------------------------------------------------------------------------------- GPU
 def matrix(R, K, dtype, seed, spread=1.0):
     g = torch.Generator().manual_seed(seed)
@@ -627,3 +651,120 @@ def test_autograd_sees_that_an_output_was_written():
     with torch.inference_mode():
         buf = torch.zeros(40, 64, device="cuda")
     assert torch.equal(ops.mxfp4_linear(a, W, out=buf), ops.mxfp4_linear(a, W))
+
+
+# The forms that the cases above leave out.  Tiles of 256 x 256 whose rows are whole lines of 128 bytes, several for every
+# workgroup; rows of at least four stages that end in half a stage, whatever the kernel.
+WHOLE_LINES = [(2048, 30208), (2100, 30208), (2048, 30016), (2100, 30016)]  # (rows and columns that fill their tiles, or do not)
+LONG_ROUTES = [(40, 300), (100, 5100), (3, 90001), (50, 41003), (500, 23001), (520, 40001), (40, 300)]
+
+
+def long_cases():
+    return [(N, M, 1100) for N, M in LONG_ROUTES[:-1]] + [(N, M, 1900) for N, M in LONG_ROUTES[-1:]]
+
+
+def drawn(R, K, seed, dtype=torch.float32):
+    """As ``matrix``, made on the GPU (large ones)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(R, K, generator=g, device="cuda")
+    return (x * torch.exp(torch.randn(R, K, generator=g, device="cuda"))).to(dtype)
+
+
+def exact_product(xq, Wq, b=None):
+    """In 64 bits, and how far fp32 accumulation may be off (the module's bound); NaN wherever a NaN goes in."""
+    xv, wv = xq.dequantize().double(), Wq.dequantize().double()
+    ref = xv @ wv.t()
+    room = xv.shape[1] * 2.0**-23 * (torch.nan_to_num(xv).abs() @ torch.nan_to_num(wv).abs().t())
+    if b is not None:
+        ref = ref + b.double()
+        room = room + 2.0**-24 * ref.abs()
+    return ref, room
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [64, 300, 512, 700])
+@pytest.mark.parametrize("N,M", WHOLE_LINES)
+def test_linear_whole_lines(N, M, K):
+    """Every form of the large kernel: both types, with and without ReLU, no bias or one of either type."""
+    from clt_training_amd import hip_ops as ops
+
+    xq, Wq = ops.mxfp4_quantize(drawn(N, K, 1)), ops.mxfp4_quantize(drawn(M, K, 2))
+    for b in (None, drawn(1, M, 3)[0], drawn(1, M, 4, torch.bfloat16)[0]):
+        ref, room = exact_product(xq, Wq, b)
+        for relu in (False, True):
+            want = ref.clamp(min=0) if relu else ref
+            for dt in (torch.bfloat16, torch.float32):
+                assert route(N, M, K, dt) == "256 x 256"
+                y = ops.mxfp4_linear(xq, Wq, b, relu=relu, out_dtype=dt)
+                assert y.data_ptr() % 128 == 0
+                allowed = room + (torch.finfo(dt).eps / 2 if dt != torch.float32 else 0) * (ref.abs() + room)
+                bad = ((y.double() - want).abs() > allowed).nonzero()
+                assert len(bad) == 0, (b is not None and b.dtype, relu, dt, len(bad), bad[:4].tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M,K", long_cases())
+def test_linear_special_values_in_long_rows(N, M, K):
+    """NaN in every quarter of the columns and in the last, half-empty stage, rows of NaN behind rows that end there, and biases
+    that are not finite."""
+    from clt_training_amd import hip_ops as ops
+
+    x, W, b = drawn(N, K, 1), drawn(M, K, 2), drawn(1, M, 3)[0]
+    x[1] = float("nan")
+    bad_rows = [9, 21, 33, 40, 47, M - 1]
+    for r, c in zip(bad_rows, (3, K // 4 + 40, K // 2 + 40, K - 150, K - 1, K - 60)):
+        W[r, c] = float("-inf")
+    W[21], W[M - 1] = float("nan"), float("nan")
+    b[0], b[1], b[2] = float("nan"), float("inf"), float("-inf")
+    xq, Wq = ops.mxfp4_quantize(x), ops.mxfp4_quantize(W)
+    ref, room = exact_product(xq, Wq, b)
+    for relu in (False, True):
+        want = torch.where(ref < 0, 0, ref) if relu else ref
+        for given in (x, xq):
+            y = ops.mxfp4_linear(given, Wq, b, relu=relu)
+            assert torch.equal(torch.isnan(y), torch.isnan(want)) and int(torch.isnan(y).sum()) == M + (1 + len(bad_rows)) * (N - 1)
+            sure = torch.isfinite(want)
+            assert ((y.double() - want).abs() <= room)[sure].all() and torch.equal(y.double()[torch.isinf(want)], want[torch.isinf(want)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M,K", long_cases())
+def test_linear_any_alignment_in_long_rows(N, M, K):
+    """As test_linear_any_alignment_every_route."""
+    from clt_training_amd import hip_ops as ops
+
+    xs, b, Wq = drawn(N, K + 3, 4), drawn(1, M + 1, 5, torch.bfloat16)[0][1:], ops.mxfp4_quantize(drawn(M, K, 6))
+    for dt in (torch.bfloat16, torch.float32):
+        want = ops.mxfp4_linear(xs[:, 1:K + 1].contiguous(), Wq, b.clone(), relu=True, out_dtype=dt)
+        big = torch.full((N + 2, M + 9), 7.0, dtype=dt, device="cuda")
+        y = ops.mxfp4_linear(xs[:, 1:K + 1], Wq, b, relu=True, out=big[1:N + 1, 3:3 + M])
+        assert torch.equal(y, want)
+        y.fill_(7)
+        assert (big == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M,K", long_cases())
+def test_linear_two_graphs_in_long_rows(N, M, K):
+    """Two captured graphs replayed in turn, three times, with eager work between."""
+    from clt_training_amd import hip_ops as ops
+
+    W = [ops.mxfp4_quantize(drawn(M, K, 7 + i)) for i in range(2)]
+    x = [drawn(N, K, 9 + i, torch.bfloat16) for i in range(2)]
+    eager = lambda i: ops.mxfp4_linear(x[i], W[i], relu=True)  # noqa: E731
+    eager(0), eager(1)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(eager(i))
+        graphs.append(g)
+    for seed in range(3):
+        for i in range(2):
+            x[i].copy_(drawn(N, K, 20 + 2 * seed + i, torch.bfloat16))
+        want = [eager(0), eager(1)]
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
