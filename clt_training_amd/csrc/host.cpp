@@ -88,8 +88,8 @@ struct Scratch {
 };
 
 // A tensor was written in place: autograd sees that a saved value is no longer there.  (Inference tensors have no count.)
-void written(const Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+void written(c10::TensorImpl* t) {
+  if (!t->is_inference()) t->bump_version();
 }
 
 // rows of unit stride (a copy if they have another)
@@ -205,7 +205,7 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
     check(linear_fn(x_.const_data_ptr<uint8_t>(), x_scales->const_data_ptr<uint8_t>(), wc, ws, bp, bc, N, M, cols, relu,
                     out.mutable_data_ptr(), oc, ldo, on.stream),
           "clt_mxfp4_linear");
-    if (out_) written(out);
+    if (out_) written(out.unsafeGetTensorImpl());
     return out;
   }
   const Tensor x = rows_of(x_);
@@ -214,7 +214,7 @@ Tensor mxfp4_linear(const Tensor& x_, const OptTensor& x_scales, const Tensor& c
   check(linear_x_fn(x.const_data_ptr(), xc, row_stride(x), wc, ws, bp, bc, N, M, cols, relu, out.mutable_data_ptr(), oc, ldo,
                     scratch.p, bytes, on.stream),
         "clt_mxfp4_linear_x");
-  if (out_) written(out);
+  if (out_) written(out.unsafeGetTensorImpl());
   return out;
 }
 
@@ -286,6 +286,9 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   std::vector<Tensor> keep;  // contiguous copies outlive the launch
   Ranges memory;
   memory.all.reserve(6 * n);
+  std::vector<std::pair<Tensor, Tensor>> pairs;  // (a sequence may make its items when it is asked for them)
+  std::vector<c10::TensorImpl*> changed;         // (held by the lists and by `pairs`)
+  changed.reserve(5 * n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params.tensor(i);
     const bool dense = grads.tensor(i).is_contiguous();
@@ -312,8 +315,10 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
                           ": moments of the parameter's shape, contiguous, on ", dev);
         ptr[k] = c.mutable_data_ptr();
         memory.add(ptr[k], 4 * numel, true);
+        changed.push_back(c.unsafeGetTensorImpl());
       } else {
-        const auto pair = py::handle(o).cast<std::pair<Tensor, Tensor>>();
+        pairs.push_back(py::handle(o).cast<std::pair<Tensor, Tensor>>());
+        const auto& pair = pairs.back();
         const auto ct = pair.first.scalar_type(), st = pair.second.scalar_type();
         TORCH_CHECK_TYPE((ct == at::kByte || ct == at::kFloat8_e4m3fn) && (st == at::kByte || st == at::kFloat8_e8m0fnu),
                          "adamw_step: tensor ", i, ": 8-bit moments are uint8 / float8_e4m3fn codes with uint8 / "
@@ -324,6 +329,8 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
                           "adamw_step: tensor ", i, ": one code per element and one scale per 128, contiguous, on ", dev);
         ptr[k] = pair.first.mutable_data_ptr();
         (k ? r.v_scale : r.m_scale) = static_cast<uint8_t*>(pair.second.mutable_data_ptr());
+        changed.push_back(pair.first.unsafeGetTensorImpl());
+        changed.push_back(pair.second.unsafeGetTensorImpl());
         memory.add(ptr[k], numel, true);
         memory.add(k ? r.v_scale : r.m_scale, (numel + 127) / 128, true);
       }
@@ -332,23 +339,14 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     r.numel = numel, r.lr = lrs[i], r.weight_decay = wds[i];
     r.p_dtype = p.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
     r.g_dtype = g.scalar_type() == at::kFloat ? CLT_F32 : CLT_BF16;
+    changed.push_back(p.unsafeGetTensorImpl());
     memory.add(r.p, numel * p.element_size(), true);
     memory.add(r.g, numel * g.element_size(), false);
   }
   TORCH_CHECK_VALUE(!memory.clash(), "adamw_step: a tensor is given twice, or two share memory (parameters and moments are "
                     "updated in place)");
   check(adamw_fn(table.data(), (int)n, betas.first, betas.second, eps, step, (uint32_t)seed, on.stream), "clt_adamw_step");
-  for (size_t i = 0; i < n; ++i) {
-    written(params.tensor(i));
-    for (PyObject* o : {first[i], second[i]}) {
-      if (THPVariable_Check(o)) {
-        written(THPVariable_Unpack(o));
-      } else {
-        const auto pair = py::handle(o).cast<std::pair<Tensor, Tensor>>();
-        written(pair.first), written(pair.second);
-      }
-    }
-  }
+  for (c10::TensorImpl* t : changed) written(t);
 }
 
 }  // namespace
