@@ -4,7 +4,7 @@
 //   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // HBM-bound: per element 2 sizeof(p) + sizeof(g) bytes of parameter and gradient plus 16 (fp32 moments) or 4 + 4/128 (8-bit
-// moments).  Measured on four 98304 x 768 bf16 tables with bf16 gradients: 1.22 ms, 5.45 TB/s (fp32 moments), 0.53 ms, 5.7 TB/s
+// moments).  Measured on four 98304 x 768 bf16 tables with bf16 gradients: 1.22 ms, 5.46 TB/s (fp32 moments), 0.53 ms, 5.74 TB/s
 // (8-bit moments); a large copy reaches 4.9 TB/s here.  The 8-bit path is near the vector units' limit, too: with the
 // stochastic rounding written out in integer arithmetic instead of the hardware's conversion it took 0.61 ms.  One launch takes
 // up to MAX_TENSORS tensors, whose records travel in the kernel's arguments: no table in device memory, so nothing is uploaded,
@@ -16,8 +16,7 @@
 // Rounding is stochastic: with b2 = 0.999 r changes by 0.05 % a step and half a step of e4m3 is 3 to 6 %, so rounding to
 // nearest would freeze it.  The 16 random bits per value are a hash of (seed, tensor, step, element): the same call gives
 // the same bits.  r > 0 is never rounded to 0 (the update m / r would jump to m / eps); v is formed in fp32, so r is 0 where v is
-// below 2^-150.  A NaN or infinite value is
-// stored as NaN and does not count for its block's scale.
+// below 2^-150.  A NaN or infinite value is stored as NaN and does not count for its block's scale.
 #include <math.h>
 
 #include "common.h"
@@ -27,7 +26,8 @@ namespace {
 
 constexpr int MAX_TENSORS = 40;   // records in one launch's arguments (40 x 88 bytes: the argument segment holds 4 KiB)
 constexpr int VEC = 8;            // elements per lane and pass
-constexpr int CHUNK = 256 * VEC;  // elements per workgroup (twice as many: +3 %, four times: +9 % on 302 M elements)
+// Elements per workgroup: one pass.  (Two passes: +3 % with fp32 and +6 % with 8-bit moments, four: +4 and +11 %, 302 M elements.)
+constexpr int CHUNK = 256 * VEC;
 constexpr int BLOCK8 = 128;       // elements per scale
 constexpr int64_t MAX_CHUNKS = (1 << 24) - 1;  // workgroups of a launch (its threads are counted in 32 bits)
 
@@ -53,7 +53,9 @@ struct Args {
 };
 static_assert(sizeof(Args) <= 4096, "kernel arguments");
 
-__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {  // two rounds of xor-shift and multiply
+// Two rounds of xor-shift and multiply, a permutation of 32 bits; shifts and factors are a set of low bias that the public
+// "hash prospector" search for such mixers lists.
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   x = (x ^ (x >> 16)) * 0x21F0AAADu;
   x = (x ^ (x >> 15)) * 0x735A2D97u;
   return x ^ (x >> 15);
@@ -63,8 +65,10 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // Eight elements from an address with no more than the element's own alignment (gfx950 takes dword loads at any byte), each
-// read and written once.  (Non-temporal stores, plain loads: 5.47 and 4.87 TB/s with fp32 and 8-bit moments of bf16 tables; both
-// non-temporal 5.29 and 4.95, loads only 5.19 and 4.77, neither 5.48 and 4.80.)
+// read and written once.  TB/s with fp32 moments and with 8-bit moments of four 98304 x 768 bf16 tables, and with 8-bit moments of
+// three 4099 x 769 fp32 tables:
+//   stores non-temporal, loads plain (this): 5.46, 5.74, 5.3    both non-temporal: 5.29, 5.96, 4.9
+//   loads non-temporal, stores plain:        5.21, 5.45, 4.9    both plain:        5.49, 5.61, 5.4
 template <typename T>
 struct Vec8;
 template <>
@@ -257,7 +261,8 @@ __device__ __forceinline__ void chunk(const Rec& t, const Args& a, int64_t start
   }
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
-    // 1-ulp square root and reciprocal: the update they feed is a small part of p, and r is rounded to 4 bits
+    // 1-ulp square root and reciprocal: the update they feed is a small part of p, and r is rounded to 4 bits (of 18.6 million
+    // stored codes 2 differ from those of 64-bit arithmetic; of a form with correctly rounded fp32 roots 3 did)
     const float upd = m[q] * __builtin_amdgcn_rcpf(fmaf(r[q], a.inv_sqrt_bc2, a.eps));
     p[q] = fmaf(-t.step_size, upd, p[q] * t.decay);
   }

@@ -143,8 +143,8 @@ struct LinearArgs {
 };
 
 // 16 bytes of a row to an address with the element's own alignment.  LINES: the row's pieces of 128 bytes are whole lines, and
-// go past L2, where the operands stay (8192 tokens x 98304 x 768, bf16: 552 us, through L2 605; fp32 649, 821).  Else through
-// L2, which joins the parts of a line (2048 x 43579 x 64: 42 us, past it 102).
+// go past L2, where the operands stay (8192 tokens x 98304 x 768, bf16: 457 us, through L2 552; fp32 636, 820).  Else through
+// L2, which joins the parts of a line (2048 x 43579 x 64: 43 us, past it 103).
 typedef uint32_t u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
 template <bool LINES>
