@@ -383,6 +383,27 @@ def test_copies_go_on_where_the_optimizer_stands(monkeypatch):
         assert sorted(calls) == [(1, False, 2, 0.1, 6), (1, True, 3, 0.1, 6)] and new._step == 3 and opt._step == 2
 
 
+def test_trainer_resumes_every_parameters_count(tmp_path):
+    """Counts that differ go through a trainer's checkpoint."""
+    from clt_training_amd import SparseCoderConfig, TrainConfig, Trainer
+
+    def trainer():
+        cfg = TrainConfig(sae=SparseCoderConfig(k=4, expansion_factor=2, transcode=True), hookpoints=["a"], optimizer="adamw")
+        return Trainer(cfg, [None] * 10, device="cpu", input_widths={"a": 8})
+
+    first = trainer()
+    opt = first.optimizers[0]
+    params = [p for g in opt.param_groups for p in g["params"]]
+    for i, p in enumerate(params[:-1]):  # (the last one never had a gradient)
+        opt._moments(p)
+        opt._steps[p] = 3 + i % 2
+    opt._step = 4
+    first.save(tmp_path)
+    again = trainer().load_state(tmp_path).optimizers[0]
+    assert again._step == 4
+    assert [again._steps.get(p) for g in again.param_groups for p in g["params"]] == [3 + i % 2 for i in range(len(params) - 1)] + [None]
+
+
 # ---------------------------------------------------------------------------------------------------------------- GPU
 SIZES = [(1,), (7,), (8,), (127,), (128,), (129,), (16, 8), (8191,), (8192,), (8193,), (33, 65), (257, 769)]
 
